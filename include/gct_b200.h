@@ -38,6 +38,10 @@ extern "C" {
 #define GCT_F32 0
 #define GCT_BF16 1
 
+/* How a manager's cache is held (gct_mgr_set_kv_format). */
+#define GCT_KV_BF16 0
+#define GCT_KV_FP4 1 /* 4-bit values with a scale for 16 of them: 36 bytes a row of 64 */
+
 #define GCT_ROPE_NONE 0
 #define GCT_ROPE_2D 1 /* rotate-half inside each 32-wide half: lingbot_map/layers/rope.py:134-198 */
 #define GCT_ROPE_3D 2 /* interleaved pairs (2m,2m+1): lingbot_map/layers/rope.py:435-461 */
@@ -73,6 +77,21 @@ int gct_version(void);
 /* FlashInferKVCacheManager.__init__ (flashinfer_cache.py:75-196), minus allocation. */
 int gct_mgr_create(gct_mgr_t** out, const gct_mgr_config_t* cfg, gct_mgr_geometry_t* geo_out);
 int gct_mgr_destroy(gct_mgr_t* m);
+
+/* Hold the cache in another format than bf16 (no counterpart in the reference); before gct_mgr_bind.  geo_out (optional) receives the
+ * geometry with the size of a pool in that format.
+ * GCT_KV_FP4: a pool is [max_num_pages][2 (K,V)][H] regions of pool_bytes / (max_num_pages * 2 * H) bytes, 16-byte aligned.  A region holds a
+ * page's rows of one head in blocks of 128 (the last one rounded up to a multiple of 4 rows): the block's packed values, 32 bytes a row,
+ * the lower four bits of a byte first, then its scales, 4 bytes a row.  A row's sixteen values number 16 i ... 16 i + 15 stand for scale i times a
+ * 4-bit number: sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6 for 0 ... 7.  A scale is a byte of five exponent and three mantissa bits, without
+ * sign: byte << 7 is the scale as a half-precision number.  K and V are rounded
+ * to bf16 as the other format stores them; a scale is the largest absolute value of its sixteen over 6, rounded to the nearest with
+ * ties to even, at most 10240 (larger values saturate at 61440); a value is x / scale rounded to the nearest of the eight, ties to the one
+ * with an even number.  Sixteen values of which one is not finite get the scale 0xff, a NaN, and all sixteen read as NaN.
+ * Every call on the manager takes either format, except that gct_mgr_read_frame_fp4 and gct_mgr_read_page_fp4 read the 4-bit one only.
+ * Rows that no append has written are never multiplied with: a 4-bit pool needs no initialisation (gct_mgr_scan_keys, which reads whole
+ * pools, wants them written or zero). */
+int gct_mgr_set_kv_format(gct_mgr_t* m, int format, gct_mgr_geometry_t* geo_out);
 
 /* Hand the manager the caller-allocated device memory: one bf16 pool per block laid out
  * [max_num_pages, 2 (K,V), page_size, H, 64] (flashinfer_cache.py:141-148) and a workspace for
@@ -154,6 +173,13 @@ int gct_mgr_attention(gct_mgr_t* m, int block, const void* q_dev, int q_dtype, i
  * Used when partial results over a page sub-range are merged across GPUs. */
 int gct_mgr_attention_partial(gct_mgr_t* m, int block, const void* q_dev, int q_dtype, int n_q,
                               float* out_f32_dev, float* lse_dev, void* stream);
+
+/* What a 4-bit cache holds of the newest frame (specials first, as it was appended; its patches must still be cached): values
+ * [tokens_per_frame, H, 64] as e4m3 bytes and scales [tokens_per_frame, H, 4] in half precision, of K and of V. */
+int gct_mgr_read_frame_fp4(gct_mgr_t* m, int block, uint8_t* k_values_dev, void* k_scales_dev, uint8_t* v_values_dev, void* v_scales_dev,
+                           void* stream);
+/* The first `rows` rows of a page of a 4-bit cache as bf16 [rows, H, 64] (exact: a value times its scale is a bf16 number). */
+int gct_mgr_read_page_fp4(gct_mgr_t* m, int block, int page, int rows, void* k_out_dev, void* v_out_dev, void* stream);
 
 /* Reads the device status word (blocks on `stream`): 0 if no kernel reported a problem. */
 int gct_mgr_device_status(gct_mgr_t* m, void* stream, int* status_out);
@@ -250,6 +276,23 @@ int gct_decode_workspace_bytes(int heads, int head_dim, size_t* bytes_out);
 int gct_decode_attention(const float* q_dev, const float* k_new_dev, const float* v_new_dev, int n_new,
                          float* cache_k_dev, float* cache_v_dev, int cached, int capacity, int store, int heads,
                          int head_dim, float* out_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* The same on a cache held in 4 bits (no counterpart in the reference).  cache_k_dev / cache_v_dev: [H][capacity / 128] blocks of 128
+ * rows each, head_dim / 2 * 128 bytes of values and head_dim / 16 * 128 bytes of scales as GCT_KV_FP4 above describes them, quantised from
+ * the fp32 rows; capacity is a multiple of 128, gct_decode_fp4_sizes gives the bytes of either cache.  n_new: any number of new tokens;
+ * they are quantised before they are attended to, stored or not.  q, out and the arithmetic are fp32 (products of q and of the weights in
+ * two half-precision parts: about 2^-21).  The workspace must be zero before the first call; its first word is a status word as
+ * gct_mgr_device_status reports it. */
+int gct_decode_fp4_sizes(int heads, int head_dim, int capacity, size_t* cache_bytes_out, size_t* workspace_bytes_out);
+int gct_decode_attention_fp4(const float* q_dev, const float* k_new_dev, const float* v_new_dev, int n_new, uint8_t* cache_k_dev,
+                             uint8_t* cache_v_dev, int cached, int capacity, int store, int heads, int head_dim, float* out_dev,
+                             void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Store `rows` rows [rows, H, D] at row `first` without attending to anything. */
+int gct_decode_append_fp4(const float* k_dev, const float* v_dev, int rows, uint8_t* cache_k_dev, uint8_t* cache_v_dev, int first,
+                          int capacity, int heads, int head_dim, void* stream);
+/* Rows [first, first + rows) as values [rows, H, D] in e4m3 bytes and scales [rows, H, D / 16] in half precision. */
+int gct_decode_read_fp4(const uint8_t* cache_k_dev, const uint8_t* cache_v_dev, int first, int rows, int capacity, int heads, int head_dim,
+                        uint8_t* k_values_dev, void* k_scales_dev, uint8_t* v_values_dev, void* v_scales_dev, void* stream);
 
 /* ---- point-cloud helpers of the offline renderer (compute only) ---------------------------- */
 

@@ -13,6 +13,7 @@ GCT_OK = 0
 ERR_INVALID, ERR_POOL_EXHAUSTED, ERR_UNDERFLOW, ERR_CUDA, ERR_DEVICE_STATUS, ERR_CAPACITY = 1, 2, 3, 4, 5, 6
 F32, BF16 = 0, 1
 ROPE_NONE, ROPE_2D, ROPE_3D = 0, 1, 2
+KV_BF16, KV_FP4 = 0, 1
 
 
 class GctError(RuntimeError):
@@ -40,6 +41,7 @@ SIGNATURES = {
     "gct_last_error": (C.c_char_p, []),
     "gct_version": (_i, []),
     "gct_mgr_create": (_i, [C.POINTER(_vp), C.POINTER(MgrConfig), C.POINTER(MgrGeometry)]),
+    "gct_mgr_set_kv_format": (_i, [_vp, _i, C.POINTER(MgrGeometry)]),
     "gct_mgr_destroy": (_i, [_vp]),
     "gct_mgr_bind": (_i, [_vp, C.POINTER(_vp), _vp, _sz]),
     "gct_mgr_workspace_bytes": (_i, [_vp, C.POINTER(_sz)]),
@@ -60,6 +62,8 @@ SIGNATURES = {
     "gct_mgr_plan": (_i, [_vp, _i, _i, _vp]),
     "gct_mgr_attention": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _vp]),
     "gct_mgr_attention_partial": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _vp]),
+    "gct_mgr_read_frame_fp4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp]),
+    "gct_mgr_read_page_fp4": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "gct_mgr_device_status": (_i, [_vp, _vp, _pi]),
     "gct_mgr_launch_count": (_i, [_vp, _pi64]),
     "gct_mgr_kernel_timing": (_i, [_vp, _i]),
@@ -77,6 +81,10 @@ SIGNATURES = {
                                         _i, _i, _vp]),
     "gct_decode_workspace_bytes": (_i, [_i, _i, C.POINTER(_sz)]),
     "gct_decode_attention": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
+    "gct_decode_fp4_sizes": (_i, [_i, _i, _i, C.POINTER(_sz), C.POINTER(_sz)]),
+    "gct_decode_attention_fp4": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
+    "gct_decode_append_fp4": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "gct_decode_read_fp4": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "gct_frustum_cull": (_i, [_vp, _i64, C.POINTER(C.c_float), C.POINTER(C.c_float), C.c_float, C.c_float, C.c_float,
                               C.c_float, _i, _i, C.c_float, C.c_float, _vp, _vp]),
     "gct_voxel_morton": (_i, [_vp, _vp, C.c_float, _i64, _vp, _vp, _vp, _vp]),

@@ -23,11 +23,25 @@ _native = _lib.binding()
 
 
 class DecodeCache:
-    """K and V rows of one (refinement iteration, block) pair: [capacity, H, D] fp32, `count` rows valid."""
+    """K and V rows of one (refinement iteration, block) pair: [capacity, H, D] fp32, `count` rows valid.
 
-    def __init__(self, heads: int, head_dim: int, device, capacity: int = 1024):
+    With kv_bits=4 the rows are held in 4-bit values with a scale for 16 of them (include/gct_b200.h, gct_decode_attention_fp4): `k` and
+    `v` are uint8 [H, capacity / 128, bytes of 128 rows], 0.14 of the memory; queries, new rows, outputs and arithmetic stay fp32."""
+
+    def __init__(self, heads: int, head_dim: int, device, capacity: int = 1024, kv_bits: int = 32):
+        if kv_bits not in (32, 4):
+            raise ValueError(f"kv_bits must be 32 (fp32) or 4, got {kv_bits!r}")
         self.heads, self.head_dim, self.device = heads, head_dim, torch.device(device)
+        self.kv_bits = kv_bits
         self.count = 0
+        if kv_bits == 4:
+            cache, work = C.c_size_t(), C.c_size_t()
+            blocks = max(-(-int(capacity) // 128), 1)
+            _lib.check(_lib.load().gct_decode_fp4_sizes(heads, head_dim, blocks * 128, C.byref(cache), C.byref(work)))
+            shape = (heads, blocks, cache.value // (heads * blocks))
+            self.k, self.v = (torch.zeros(shape, dtype=torch.uint8, device=self.device) for _ in range(2))
+            self.workspace = torch.zeros(work.value, dtype=torch.uint8, device=self.device)
+            return
         self.k = torch.zeros(capacity, heads, head_dim, dtype=torch.float32, device=self.device)
         self.v = torch.zeros(capacity, heads, head_dim, dtype=torch.float32, device=self.device)
         need = C.c_size_t()
@@ -36,12 +50,19 @@ class DecodeCache:
 
     @property
     def capacity(self) -> int:
-        return self.k.shape[0]
+        return self.k.shape[1] * 128 if self.kv_bits == 4 else self.k.shape[0]
 
     def _grow(self, rows: int) -> None:
         cap = self.capacity
         while cap < rows:
             cap *= 2
+        if self.kv_bits == 4:
+            for name in ("k", "v"):
+                old = getattr(self, name)
+                new = torch.zeros(self.heads, cap // 128, old.shape[2], dtype=torch.uint8, device=self.device)
+                new[:, :old.shape[1]].copy_(old)
+                setattr(self, name, new)
+            return
         for name in ("k", "v"):
             old = getattr(self, name)
             new = torch.zeros(cap, self.heads, self.head_dim, dtype=torch.float32, device=self.device)
@@ -54,7 +75,9 @@ class DecodeCache:
         n = q.shape[0]
         if store and self.count + n > self.capacity:
             self._grow(self.count + n)
-        if n <= 8:
+        if self.kv_bits == 4:
+            out = _native.decode_attention_fp4(q, k_new, v_new, self.k, self.v, self.count, store, self.workspace)
+        elif n <= 8:
             out = _native.decode_attention(q, k_new, v_new, self.k, self.v, self.count, store, self.workspace)
         else:
             # a scale phase of more than 8 frames: the kernel takes 8 query tokens per launch.  Each chunk of
@@ -74,6 +97,36 @@ class DecodeCache:
         if store:
             self.count += n
         return out
+
+
+    def append(self, k: Tensor, v: Tensor) -> None:
+        """Store rows k, v [n, H, D] fp32 without attending to anything (a cache restored, or filled in one go)."""
+        n = k.shape[0]
+        if tuple(k.shape) != (n, self.heads, self.head_dim) or k.shape != v.shape:
+            raise ValueError(f"k and v must be [n, {self.heads}, {self.head_dim}]")
+        if self.count + n > self.capacity:
+            self._grow(self.count + n)
+        if self.kv_bits == 4:
+            _native.decode_append_fp4(k, v, self.k, self.v, self.count)
+        else:
+            self.k[self.count:self.count + n].copy_(k)
+            self.v[self.count:self.count + n].copy_(v)
+        self.count += n
+
+    def truncate(self, count: int) -> None:
+        """Keep the first `count` rows."""
+        if not 0 <= count <= self.count:
+            raise ValueError(f"cannot keep {count} of {self.count} rows")
+        self.count = count
+
+    def rows_fp4(self, first: int, rows: int):
+        """What a 4-bit cache holds of rows [first, first + rows): (K values [rows, H, D] float8_e4m3fn, K scales [rows, H, D / 16] float16,
+        V values, V scales); scale i times values 16 i ... 16 i + 15 of a row are what the attention multiplies with."""
+        if self.kv_bits != 4:
+            raise ValueError("the cache is not held in 4 bits")
+        if not 0 <= first <= first + rows <= self.count:
+            raise ValueError(f"rows [{first}, {first + rows}) of {self.count}")
+        return _native.decode_read_fp4(self.k, self.v, self.head_dim, first, rows)
 
 
 def _reference_causal_attention():
@@ -119,7 +172,7 @@ class B200CausalAttention(torch.nn.Module):
         key = f"b200_decode_{global_idx}"
         cache = kv_cache.get(key)
         if cache is None:
-            cache = kv_cache[key] = DecodeCache(H, D, x.device)
+            cache = kv_cache[key] = DecodeCache(H, D, x.device, kv_bits=getattr(self, "b200_kv_bits", 32))
         nhd = lambda t: t[0].permute(1, 0, 2).float().contiguous()          # [N, H, D] fp32
         store = not kv_cache.get("_skip_append", False)                    # attention.py:232-249
         out = cache.attend(nhd(q), nhd(k), nhd(v), store)                  # [N, H, D]
@@ -130,13 +183,16 @@ class B200CausalAttention(torch.nn.Module):
         return self.proj_drop(self.proj(out))
 
 
-def convert_camera_head(head) -> int:
-    """Switch the attention modules of a CameraCausalHead's trunk (camera_head.py:221-228) to B200CausalAttention.
-    Returns how many were converted."""
+def convert_camera_head(head, kv_bits: int = 32) -> int:
+    """Switch the attention modules of a CameraCausalHead's trunk (camera_head.py:221-228) to B200CausalAttention, whose caches are held
+    in fp32 or (kv_bits=4) in 4 bits.  Returns how many were converted."""
+    if kv_bits not in (32, 4):
+        raise ValueError(f"kv_bits must be 32 (fp32) or 4, got {kv_bits!r}")
     n = 0
     for blk in getattr(head, "trunk", []):
         attn = getattr(blk, "attn", None)
         if attn is not None and hasattr(attn, "qkv") and hasattr(attn, "gate_proj") and not isinstance(attn, B200CausalAttention):
             attn.__class__ = B200CausalAttention
+            attn.b200_kv_bits = kv_bits
             n += 1
     return n

@@ -148,6 +148,10 @@ struct PrepLaunch {
   __nv_bfloat16* k_out = nullptr; __nv_bfloat16* v_out = nullptr;
   // K/V destination, paged (k_out == null): pool [pages, 2, page_size, H, 64]
   __nv_bfloat16* pool = nullptr;
+  // or a 4-bit pool [pages, 2, H, pool4_head_bytes] (gct_fp4.h), with the blocks of a page
+  uint8_t* pool4 = nullptr;
+  int64_t pool4_head_bytes = 0;
+  int pool4_full_blocks = 0, pool4_tail_rows = 0;
   int page_size = 0, num_pages = 0, num_special = 0;
   PageSlots dst[kAppendFrames];      // of frame token / tokens_per_frame
   int* status = nullptr;
@@ -199,6 +203,10 @@ int launch_residual_norm(const RowLaunch& p, cudaStream_t stream);
 int launch_gelu(__nv_bfloat16* x, int64_t n, cudaStream_t stream);
 // Table of the 2-D rotation [tokens, 32, 2] from integer positions [tokens, 2] with the given strides.
 int launch_rope2d_positions(const int64_t* pos, int64_t token_stride, int64_t axis_stride, int tokens, float base, float* cs, cudaStream_t stream);
+
+// Rows of the newest frame of a 4-bit cache (e4m3 values and half-precision scales, K then V), and of one page as bf16.
+int mgr_read_frame_fp4(gct_mgr_t* m, int block, uint8_t* const values[2], void* const scales[2], cudaStream_t stream);
+bool mgr_is_fp4(const gct_mgr_t* m);
 
 // key_norm_max[head] = max over all K rows of the pool [pages, 2, page_size, heads, 64] of their 2-norm
 int launch_scan_keys(const __nv_bfloat16* pool, int num_pages, int page_size, int heads, float* key_norm_max,

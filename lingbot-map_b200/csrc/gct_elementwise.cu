@@ -4,7 +4,7 @@
 
 #include <type_traits>
 
-#include "gct_common.h"
+#include "gct_fp4.h"
 
 namespace gct {
 namespace {
@@ -170,8 +170,31 @@ __device__ __forceinline__ void rotate16(float (&x)[16], const float2 (&cs)[8]) 
   }
 }
 
-// kMode: rotation; kQkF32, kVF32: types of the sources of q and k, and of v.
-template <int kMode, bool kQkF32, bool kVF32>
+// A lane's sixteen elements as they go into a 4-bit cache: the values a bf16 cache would hold, quantised (gct_fp4.h).  The lanes s and
+// s ^ 1 hold the halves of two blocks of 16, [32 (s / 2), +16) and the next; each takes over the other's half of one, so that lane s ends up
+// with block s: eight bytes and a scale byte.
+__device__ __forceinline__ uint32_t fp4_block16(const float (&x)[16], int part, uint32_t (&w)[2]) {
+  float b[16];
+  uint32_t top0 = 0, top1 = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) b[i] = __bfloat162float(__float2bfloat16_rn(x[i]));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    top0 = max(top0, fp4_abs_bits(b[i]));
+    top1 = max(top1, fp4_abs_bits(b[8 + i]));
+  }
+  const uint32_t byte0 = fp4_scale_byte(max(top0, __shfl_xor_sync(0xffffffffu, top0, 1)));
+  const uint32_t byte1 = fp4_scale_byte(max(top1, __shfl_xor_sync(0xffffffffu, top1, 1)));
+  const uint32_t w0 = fp4_pack8(b, fp4_scale(byte0)), w1 = fp4_pack8(b + 8, fp4_scale(byte1));
+  const bool odd = part & 1;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
+  w[0] = odd ? other : w0;
+  w[1] = odd ? w1 : other;
+  return odd ? byte1 : byte0;
+}
+
+// kMode: rotation; kQkF32, kVF32: types of the sources of q and k, and of v; kFp4: K and V go into a 4-bit cache.
+template <int kMode, bool kQkF32, bool kVF32, bool kFp4>
 __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch p) {
   __shared__ __align__(16) float s_norm[4][kHeadDim];       // q weight, q bias, k weight, k bias
   const int part = threadIdx.x & 3, e0 = 32 * (part >> 1) + 8 * (part & 1);
@@ -180,7 +203,7 @@ __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch
   const bool active = row < rows;           // inactive lanes (all four of a row) still take part in the shuffles
   const int r = active ? row : rows - 1;
   const int token = r / p.heads, h = r - token * p.heads;
-  const bool do_q = p.q_src != nullptr && p.q_out != nullptr, do_kv = p.k_out != nullptr || p.pool != nullptr;
+  const bool do_q = p.q_src != nullptr && p.q_out != nullptr, do_kv = kFp4 || p.k_out != nullptr || p.pool != nullptr;
   const size_t src = static_cast<size_t>(token) * p.src_token_stride + static_cast<size_t>(h) * p.src_head_stride + e0;
   pdl_wait();
   RawRow<kQkF32> rq, rk;
@@ -227,10 +250,12 @@ __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch
   // destination rows of K and V for this token
   __nv_bfloat16* k_row = nullptr;
   __nv_bfloat16* v_row = nullptr;
-  if (p.k_out != nullptr) {
+  uint8_t *k4 = nullptr, *v4 = nullptr;     // 4-bit: the lane's block of the row, its scale `scale_off` bytes further on
+  int64_t scale_off = 0;
+  if (!kFp4 && p.k_out != nullptr) {
     k_row = p.k_out + static_cast<size_t>(token) * p.heads * kHeadDim;
     v_row = p.v_out + static_cast<size_t>(token) * p.heads * kHeadDim;
-  } else if (p.pool != nullptr) {
+  } else if (kFp4 || p.pool != nullptr) {
     int page, slot;
     const int frame = token < p.tokens_per_frame ? 0 : token / p.tokens_per_frame, in_frame = token - frame * p.tokens_per_frame;
     const PageSlots& to = p.dst[frame];
@@ -246,13 +271,18 @@ __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch
     }
     if (page < 0 || page >= p.num_pages || slot < 0 || slot >= p.page_size) {
       if (active && part == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+    } else if constexpr (kFp4) {
+      const Fp4At at = fp4_at<kHeadDim>(slot, p.pool4_full_blocks, p.pool4_tail_rows);
+      k4 = p.pool4 + (static_cast<int64_t>(page) * 2 * p.heads + h) * p.pool4_head_bytes + at.values + 8 * part;
+      v4 = k4 + p.heads * p.pool4_head_bytes;
+      scale_off = at.scales + part - (at.values + 8 * part);
     } else {
       const size_t page_elems = static_cast<size_t>(p.page_size) * p.heads * kHeadDim;
       k_row = p.pool + (static_cast<size_t>(page) * 2) * page_elems + static_cast<size_t>(slot) * p.heads * kHeadDim;
       v_row = k_row + page_elems;
     }
   }
-  const bool in_range = !do_kv || k_row != nullptr;         // a token without a valid page writes nothing
+  const bool in_range = !do_kv || k_row != nullptr || k4 != nullptr;         // a token without a valid page writes nothing
 
   const size_t dst = static_cast<size_t>(h) * kHeadDim + e0;
   float x[16];
@@ -266,7 +296,28 @@ __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch
     rk.floats(x);
     if (p.kn_w != nullptr) norm16(x, s_norm[2] + e0, s_norm[3] + e0);
     rotate16<kMode>(x, cs);
-    if (active && in_range) store16(k_row + dst, x);
+    if constexpr (kFp4) {
+      uint32_t w[2];
+      const uint32_t byte = fp4_block16(x, part, w);
+      if (active && in_range) {
+        *reinterpret_cast<uint2*>(k4) = make_uint2(w[0], w[1]);
+        k4[scale_off] = static_cast<uint8_t>(byte);
+      }
+      if (p.key_norm_max != nullptr) {       // the norm is that of the row that the cache now stands for
+        uint32_t c[8];
+        fp4_unpack8(w[0], *reinterpret_cast<uint32_t(*)[4]>(&c[0]));
+        fp4_unpack8(w[1], *reinterpret_cast<uint32_t(*)[4]>(&c[4]));
+        const float s = fp4_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[i]));
+          x[2 * i] = f.x * s;
+          x[2 * i + 1] = f.y * s;
+        }
+      }
+    } else {
+      if (active && in_range) store16(k_row + dst, x);
+    }
     if (p.key_norm_max != nullptr) {
       // running maximum of |k| per head (an upper bound: fp32 values, inflated for the bf16 rounding).  Positive
       // floats order like their bit patterns; the look at the maximum above keeps atomics rare once it settles.
@@ -278,7 +329,16 @@ __global__ void __launch_bounds__(kPrepThreads) gct_prep_kernel(const PrepLaunch
         atomicMax(reinterpret_cast<unsigned int*>(p.key_norm_max + h), nrm == nrm ? __float_as_uint(nrm) : 0x7f800000u);
     }
     rv.floats(x);
-    if (active && in_range) store16(v_row + dst, x);
+    if constexpr (kFp4) {
+      uint32_t w[2];
+      const uint32_t byte = fp4_block16(x, part, w);
+      if (active && in_range) {
+        *reinterpret_cast<uint2*>(v4) = make_uint2(w[0], w[1]);
+        v4[scale_off] = static_cast<uint8_t>(byte);
+      }
+    } else {
+      if (active && in_range) store16(v_row + dst, x);
+    }
   }
 }
 
@@ -559,6 +619,37 @@ gct_scan_keys_kernel(const __nv_bfloat16* __restrict__ pool, int64_t total_rows,
   }
 }
 
+// The same for a 4-bit pool [pages, 2, heads, head_bytes]: a CTA takes one head of one page, a thread a row at a time.
+__global__ void __launch_bounds__(128)
+gct_scan_keys_fp4_kernel(const uint8_t* __restrict__ pool, int page_size, int heads, int64_t head_bytes, int full_blocks, int tail_rows, float* key_norm_max) {
+  const int h = blockIdx.x % heads;
+  const int64_t page = blockIdx.x / heads;
+  const uint8_t* base = pool + (page * 2 * heads + h) * head_bytes;
+  float top = 0.f;
+  bool bad = false;
+  for (int row = threadIdx.x; row < page_size; row += blockDim.x) {
+    const Fp4At at = fp4_at<kHeadDim>(row, full_blocks, tail_rows);
+    float sq = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint2 w = *reinterpret_cast<const uint2*>(base + at.values + 8 * g);
+      const float s = fp4_scale(base[at.scales + g]);
+      uint32_t c[8];
+      fp4_unpack8(w.x, *reinterpret_cast<uint32_t(*)[4]>(&c[0]));
+      fp4_unpack8(w.y, *reinterpret_cast<uint32_t(*)[4]>(&c[4]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[i]));
+        sq += (f.x * s) * (f.x * s) + (f.y * s) * (f.y * s);
+      }
+    }
+    const float nrm = sqrtf(sq) * 1.0001f;
+    bad |= !(nrm <= 3.0e38f);
+    top = fmaxf(top, nrm);
+  }
+  atomicMax(reinterpret_cast<unsigned int*>(key_norm_max + h), bad ? 0x7f800000u : __float_as_uint(top));
+}
+
 // cs[token][m] = (cos, sin) of the m-th complex frequency; fp64 angles as the reference's table
 // (lingbot_map/layers/rope.py:326-334,399-413): m<10 time (dim 20), m<21 height (dim 22), else width (dim 22).
 __global__ void gct_rope3d_table_kernel(int f, int pph, int ppw, int ns, float* cs) {
@@ -620,20 +711,22 @@ int launch_prep(const PrepLaunch& p, cudaStream_t stream) {
     return fail(GCT_ERR_INVALID, "prep: source strides must be multiples of 8 elements (16-byte vector loads)");
   auto misaligned = [](const void* q) { return q != nullptr && (reinterpret_cast<uintptr_t>(q) & 15) != 0; };
   if (misaligned(p.q_src) || misaligned(p.k_src) || misaligned(p.v_src) || misaligned(p.q_out) || misaligned(p.k_out) ||
-      misaligned(p.v_out) || misaligned(p.pool) || misaligned(p.qn_w) || misaligned(p.qn_b) || misaligned(p.kn_w) ||
+      misaligned(p.v_out) || misaligned(p.pool) || misaligned(p.pool4) || misaligned(p.qn_w) || misaligned(p.qn_b) || misaligned(p.kn_w) ||
       misaligned(p.kn_b) || misaligned(p.rope_cs))
     return fail(GCT_ERR_INVALID, "prep: tensors must be 16-byte aligned");
-  if (p.k_out == nullptr && p.pool != nullptr && p.tokens > static_cast<long long>(kAppendFrames) * p.tokens_per_frame)
+  if (p.k_out == nullptr && (p.pool != nullptr || p.pool4 != nullptr) && p.tokens > static_cast<long long>(kAppendFrames) * p.tokens_per_frame)
     return fail(GCT_ERR_INVALID, "prep: more frames than one launch takes");
   const long long rows = static_cast<long long>(p.tokens) * p.heads;
   if (rows > (1ll << 28)) return fail(GCT_ERR_INVALID, "prep: too many rows");
   const dim3 grid(static_cast<unsigned>((rows * 4 + kPrepThreads - 1) / kPrepThreads)), block(kPrepThreads);
   const bool qk32 = p.src_dtype_qk == GCT_F32, v32 = p.src_dtype_v == GCT_F32;
-  auto pick = [&](auto mode) {
+  auto pick_for = [&](auto mode, auto fp4) {
     constexpr int m = decltype(mode)::value;
-    return qk32 ? (v32 ? gct_prep_kernel<m, true, true> : gct_prep_kernel<m, true, false>)
-                : (v32 ? gct_prep_kernel<m, false, true> : gct_prep_kernel<m, false, false>);
+    constexpr bool f = decltype(fp4)::value;
+    return qk32 ? (v32 ? gct_prep_kernel<m, true, true, f> : gct_prep_kernel<m, true, false, f>)
+                : (v32 ? gct_prep_kernel<m, false, true, f> : gct_prep_kernel<m, false, false, f>);
   };
+  auto pick = [&](auto mode) { return p.pool4 != nullptr ? pick_for(mode, std::true_type()) : pick_for(mode, std::false_type()); };
   auto kernel = p.rope_mode == GCT_ROPE_3D ? (p.rope_f64 ? pick(std::integral_constant<int, kRope3dF64>()) : pick(std::integral_constant<int, GCT_ROPE_3D>()))
                 : p.rope_mode == GCT_ROPE_2D ? pick(std::integral_constant<int, GCT_ROPE_2D>())
                                              : pick(std::integral_constant<int, GCT_ROPE_NONE>());
@@ -702,6 +795,17 @@ int launch_scan_keys(const __nv_bfloat16* pool, int num_pages, int page_size, in
   GCT_CUDA_CHECK(cudaMemsetAsync(key_norm_max, 0, static_cast<size_t>(heads) * sizeof(float), stream));
   const int64_t total_rows = static_cast<int64_t>(num_pages) * page_size * heads;
   gct_scan_keys_kernel<<<148 * 8, 256, 0, stream>>>(pool, total_rows, page_size, heads, key_norm_max);
+  GCT_CUDA_CHECK(cudaGetLastError());
+  return GCT_OK;
+}
+
+int launch_scan_keys_fp4(const uint8_t* pool, int num_pages, int page_size, int heads, float* key_norm_max, cudaStream_t stream) {
+  if (pool == nullptr || key_norm_max == nullptr || num_pages <= 0 || page_size <= 0 || heads <= 0) return fail(GCT_ERR_INVALID, "scan_keys: bad argument");
+  const int64_t ctas = static_cast<int64_t>(num_pages) * heads;
+  if (ctas > 0x7fffffff) return fail(GCT_ERR_INVALID, "scan_keys: too many pages");
+  GCT_CUDA_CHECK(cudaMemsetAsync(key_norm_max, 0, static_cast<size_t>(heads) * sizeof(float), stream));
+  const Fp4Layout l = fp4_layout(page_size, kHeadDim);
+  gct_scan_keys_fp4_kernel<<<static_cast<unsigned>(ctas), 128, 0, stream>>>(pool, page_size, heads, l.bytes, l.full_blocks, l.tail_rows, key_norm_max);
   GCT_CUDA_CHECK(cudaGetLastError());
   return GCT_OK;
 }

@@ -5,7 +5,7 @@
 #include <mutex>
 #include <vector>
 
-#include "gct_common.h"
+#include "gct_fp4.h"
 
 namespace gct {
 
@@ -90,6 +90,12 @@ struct gct_mgr {
   bool bound = false;
   std::vector<__nv_bfloat16*> pools;
   std::vector<CUtensorMap> tm_k, tm_v;
+  // 4-bit cache (gct_mgr_set_kv_format): its pools and the blocks of a page
+  bool fp4 = false;
+  Fp4Layout fp4_page;
+  std::vector<uint8_t*> pools4;
+  int* rows_counters = nullptr;      // [kRowsCounters], zero between calls
+  size_t part_floats = 0;            // floats from part_o to the end of the workspace
   uint8_t* ws = nullptr;
   size_t ws_bytes = 0;
   int* status_dev = nullptr;
@@ -125,6 +131,7 @@ struct gct_mgr {
 
 static constexpr size_t kWsHeader = 4096;      // status word
 static constexpr int kMaxSplitsCap = 32;
+static constexpr int kRowsCounters = 4096;     // (head, eight queries) items of a split call over a 4-bit cache
 // Largest |q| * max|k| * scale * log2(e) for which the bound may stand in for the row maximum: all exponents stay
 // in [-2 * limit, 0], far inside the fp32 / bf16 exponent range.
 static constexpr float kBoundedLimit = 40.0f;
@@ -145,14 +152,15 @@ static void reset_block(const gct_mgr* m, BlockState& b) {
 static size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 struct WsLayout {
-  size_t table_off, qstage_off, parto_off, partlse_off, total_min, per_split;
+  size_t table_off, counters_off, qstage_off, parto_off, partlse_off, total_min, per_split;
 };
 static constexpr size_t kWsKeyNormOff = 256;     // key_norm_max[num_blocks][H] up to the end of the header
 static WsLayout ws_layout(const gct_mgr* m) {
   WsLayout w;
   const size_t rows = static_cast<size_t>(m->cfg.tokens_per_frame) * m->cfg.num_heads;
   w.table_off = kWsHeader;
-  w.qstage_off = align_up(w.table_off + static_cast<size_t>(m->geo.max_num_pages) * 4, 256);
+  w.counters_off = align_up(w.table_off + static_cast<size_t>(m->geo.max_num_pages) * 4, 256);
+  w.qstage_off = w.counters_off + (m->fp4 ? kRowsCounters * sizeof(int) : 0);
   w.parto_off = align_up(w.qstage_off + rows * kHeadDim * 2, 256);
   w.per_split = rows * kHeadDim * 4 + rows * 4;
   w.partlse_off = 0;
@@ -189,6 +197,18 @@ int gct_mgr_create(gct_mgr_t** out, const gct_mgr_config_t* cfg, gct_mgr_geometr
   for (auto& b : m->blocks) reset_block(m, b);
   if (geo_out != nullptr) *geo_out = m->geo;
   *out = m;
+  return GCT_OK;
+}
+
+int gct_mgr_set_kv_format(gct_mgr_t* m, int format, gct_mgr_geometry_t* geo_out) {
+  if (m == nullptr) return fail(GCT_ERR_INVALID, "null manager");
+  if (m->bound) return fail(GCT_ERR_INVALID, "gct_mgr_set_kv_format: the manager already has its pools");
+  if (format != GCT_KV_BF16 && format != GCT_KV_FP4) return fail(GCT_ERR_INVALID, "gct_mgr_set_kv_format: unknown format");
+  m->fp4 = format == GCT_KV_FP4;
+  m->fp4_page = fp4_layout(m->geo.page_size, kHeadDim);
+  const int64_t head = m->fp4 ? m->fp4_page.bytes : static_cast<int64_t>(m->geo.page_size) * kHeadDim * 2;
+  m->geo.pool_bytes = static_cast<int64_t>(m->geo.max_num_pages) * 2 * m->cfg.num_heads * head;
+  if (geo_out != nullptr) *geo_out = m->geo;
   return GCT_OK;
 }
 
@@ -257,11 +277,17 @@ int gct_mgr_bind(gct_mgr_t* m, void* const* pools_dev, void* workspace_dev, size
   if ((reinterpret_cast<uintptr_t>(workspace_dev) & 255) != 0) return fail(GCT_ERR_INVALID, "workspace must be 256-byte aligned");
   const int H = m->cfg.num_heads, P = m->geo.page_size;
   m->pools.assign(m->cfg.num_blocks, nullptr);
+  m->pools4.assign(m->cfg.num_blocks, nullptr);
   m->tm_k.resize(m->cfg.num_blocks);
   m->tm_v.resize(m->cfg.num_blocks);
   const int64_t page_elems = static_cast<int64_t>(P) * H * kHeadDim;
   for (int b = 0; b < m->cfg.num_blocks; ++b) {
     if (pools_dev[b] == nullptr) return fail(GCT_ERR_INVALID, "gct_mgr_bind: null pool");
+    if (m->fp4) {
+      if ((reinterpret_cast<uintptr_t>(pools_dev[b]) & 15) != 0) return fail(GCT_ERR_INVALID, "gct_mgr_bind: pools must be 16-byte aligned");
+      m->pools4[b] = static_cast<uint8_t*>(pools_dev[b]);
+      continue;
+    }
     m->pools[b] = static_cast<__nv_bfloat16*>(pools_dev[b]);
     int rc = make_tensor_map(&m->tm_k[b], m->pools[b], H, P, m->geo.max_num_pages, kHeadDim,
                              static_cast<int64_t>(H) * kHeadDim, 2 * page_elems);
@@ -280,7 +306,10 @@ int gct_mgr_bind(gct_mgr_t* m, void* const* pools_dev, void* workspace_dev, size
   const size_t rows = static_cast<size_t>(m->cfg.tokens_per_frame) * H;
   m->part_o = reinterpret_cast<float*>(m->ws + w.parto_off);
   m->part_lse = reinterpret_cast<float*>(m->ws + w.parto_off + static_cast<size_t>(m->max_splits) * rows * kHeadDim * 4);
+  m->part_floats = avail / sizeof(float);
+  m->rows_counters = m->fp4 ? reinterpret_cast<int*>(m->ws + w.counters_off) : nullptr;
   GCT_CUDA_CHECK(cudaMemset(m->ws, 0, kWsHeader));
+  if (m->fp4) GCT_CUDA_CHECK(cudaMemset(m->rows_counters, 0, kRowsCounters * sizeof(int)));
   const size_t kn_bytes = static_cast<size_t>(m->cfg.num_blocks) * H * sizeof(float);
   m->key_norm_max = kWsKeyNormOff + kn_bytes <= kWsHeader ? reinterpret_cast<float*>(m->ws + kWsKeyNormOff) : nullptr;
   // nothing is visible yet and the header was just zeroed: a maximum of 0 is exact
@@ -409,6 +438,10 @@ static int track_key_norms(gct_mgr* m, int block, PrepLaunch* p, cudaStream_t st
 
 static void fill_paged_dst(const gct_mgr* m, int block, const PageSlots* frames, int count, PrepLaunch* p) {
   p->pool = m->pools[block];
+  p->pool4 = m->pools4[block];
+  p->pool4_head_bytes = m->fp4_page.bytes;
+  p->pool4_full_blocks = m->fp4_page.full_blocks;
+  p->pool4_tail_rows = m->fp4_page.tail_rows;
   p->page_size = m->geo.page_size;
   p->num_pages = m->geo.max_num_pages;
   p->num_special = m->cfg.num_special_tokens;
@@ -421,8 +454,37 @@ static void fill_paged_dst(const gct_mgr* m, int block, const PageSlots* frames,
 
 }  // extern "C"
 
+extern "C" {
+static int newest_frame(const gct_mgr* m, int block, PageSlots* out);
+}
+
 namespace gct {
 const gct_mgr_config_t& mgr_config(const gct_mgr_t* m) { return m->cfg; }
+bool mgr_is_fp4(const gct_mgr_t* m) { return m->fp4; }
+
+int mgr_read_frame_fp4(gct_mgr_t* m, int block, uint8_t* const values[2], void* const scales[2], cudaStream_t stream) {
+  int rc = check_bound(m);
+  if (rc != GCT_OK) return rc;
+  if (!m->fp4) return fail(GCT_ERR_INVALID, "gct_mgr_read_frame_fp4: the cache is not held in 4 bits");
+  if (block < 0 || block >= m->cfg.num_blocks) return fail(GCT_ERR_INVALID, "gct_mgr_read_frame_fp4: block index out of range");
+  Fp4ReadLaunch p;
+  rc = newest_frame(m, block, &p.at);
+  if (rc != GCT_OK) return rc;
+  p.pool = m->pools4[block];
+  p.layout = m->fp4_page;
+  p.heads = m->cfg.num_heads;
+  p.tokens = m->cfg.tokens_per_frame;
+  p.num_special = m->cfg.num_special_tokens;
+  p.num_pages = m->geo.max_num_pages;
+  p.page_rows = m->geo.page_size;
+  for (int i = 0; i < 2; ++i) {
+    p.values[i] = values[i];
+    p.scales[i] = static_cast<__half*>(scales[i]);
+  }
+  p.status = m->status_dev;
+  m->launches += 1;
+  return launch_fp4_read(p, stream);
+}
 
 int mgr_append(gct_mgr_t* m, int block, PrepLaunch p, cudaStream_t stream) {
   int rc = check_bound(m);
@@ -572,8 +634,9 @@ int gct_mgr_scan_keys(gct_mgr_t* m, int block, void* stream) {
   if (rc != GCT_OK) return rc;
   if (block < 0 || block >= m->cfg.num_blocks) return fail(GCT_ERR_INVALID, "gct_mgr_scan_keys: block index out of range");
   if (m->key_norm_max == nullptr) return GCT_OK;       // bounded mode unavailable for this geometry
-  rc = launch_scan_keys(m->pools[block], m->geo.max_num_pages, m->geo.page_size, m->cfg.num_heads,
-                        m->key_norm_max + static_cast<size_t>(block) * m->cfg.num_heads, static_cast<cudaStream_t>(stream));
+  float* slot = m->key_norm_max + static_cast<size_t>(block) * m->cfg.num_heads;
+  rc = m->fp4 ? launch_scan_keys_fp4(m->pools4[block], m->geo.max_num_pages, m->geo.page_size, m->cfg.num_heads, slot, static_cast<cudaStream_t>(stream))
+              : launch_scan_keys(m->pools[block], m->geo.max_num_pages, m->geo.page_size, m->cfg.num_heads, slot, static_cast<cudaStream_t>(stream));
   if (rc != GCT_OK) return rc;
   m->key_norm_valid[block] = 1;
   m->key_norm_clear[block] = 0;
@@ -594,6 +657,25 @@ int gct_mgr_reset(gct_mgr_t* m) {
   // nothing is visible any more: the key-norm maxima restart from zero at the next append
   for (auto& f : m->key_norm_clear) f = 1;
   for (auto& f : m->key_norm_valid) f = 1;
+  return GCT_OK;
+}
+
+// Where the rows of the newest frame lie.
+static int newest_frame(const gct_mgr* m, int block, PageSlots* out) {
+  const BlockState& b = m->blocks[block];
+  const std::deque<int32_t>& src = b.frame_count > m->cfg.scale_frames ? b.window_pages : b.scale_pages;
+  if (b.frame_count <= 0 || src.empty()) return fail(GCT_ERR_INVALID, "block " + std::to_string(block) + ": no frame whose patches are still cached");
+  PageSlots at;
+  at.patch_page = src.back();
+  const int n = m->cfg.num_special_tokens, P = m->geo.page_size;
+  if (n > 0) {
+    const int64_t first = b.special_token_count - n;
+    at.sp_page0 = b.special_pages[first / P];
+    at.sp_off0 = static_cast<int>(first % P);
+    at.sp_n0 = std::min(n, P - at.sp_off0);
+    if (at.sp_n0 < n) at.sp_page1 = b.special_pages[first / P + 1];
+  }
+  *out = at;
   return GCT_OK;
 }
 
@@ -674,16 +756,61 @@ int gct_mgr_plan(gct_mgr_t* m, int page_begin, int page_end, void* stream) {
   return GCT_OK;
 }
 
+}  // extern "C"
+
 // Launch the attention kernel, bracketed by a CUDA-event pair when kernel timing is on.
-static int timed_attention(gct_mgr* m, const AttnLaunch& a, cudaStream_t stream) {
+template <typename F>
+static int timed(gct_mgr* m, cudaStream_t stream, F&& launch) {
   const bool t = m->timing && m->ev_used < m->ev_start.size();
   if (t) GCT_CUDA_CHECK(cudaEventRecord(m->ev_start[m->ev_used], stream));
-  const int rc = launch_attention(a, stream);
+  const int rc = launch();
   if (t) {
     GCT_CUDA_CHECK(cudaEventRecord(m->ev_stop[m->ev_used], stream));
     m->ev_used += 1;
   }
   return rc;
+}
+static int timed_attention(gct_mgr* m, const AttnLaunch& a, cudaStream_t stream) {
+  return timed(m, stream, [&] { return launch_attention(a, stream); });
+}
+
+extern "C" {
+
+// The same over a 4-bit cache; every result is final: splits_out != nullptr leaves it as the one partial result.
+static int run_paged_fp4(gct_mgr* m, int block, const void* q_dev, int q_dtype, int n_q, __nv_bfloat16* out_bf16, float* out_f32, float* lse_dev,
+                         cudaStream_t stream, int* splits_out) {
+  if (q_dtype != GCT_F32 && q_dtype != GCT_BF16) return fail(GCT_ERR_INVALID, "attention: q dtype must be GCT_F32 or GCT_BF16");
+  const int64_t rows = static_cast<int64_t>(n_q) * m->cfg.num_heads;
+  Fp4RowsLaunch p;
+  p.q = q_dev;
+  p.q_dtype = q_dtype;
+  p.q_round_bf16 = true;
+  p.n_q = n_q;
+  p.heads = m->cfg.num_heads;
+  p.pool = m->pools4[block];
+  p.page_table = m->table_dev;
+  p.n_pages = m->plan_pages;
+  p.num_pages = m->geo.max_num_pages;
+  p.page_rows = m->geo.page_size;
+  p.last_page_rows = m->plan_last_len;
+  p.layout = m->fp4_page;
+  p.out_bf16 = out_bf16;
+  p.out_f32 = out_f32;
+  p.lse = lse_dev;
+  p.part = m->part_o;
+  p.part_floats = m->part_floats;
+  p.counters = m->rows_counters;
+  p.num_counters = kRowsCounters;
+  p.status = m->status_dev;
+  if (splits_out != nullptr) {
+    *splits_out = 1;
+    p.out_f32 = m->part_o;
+    p.lse = m->part_lse;
+    p.part = m->part_o + rows * kHeadDim;
+    p.part_floats = static_cast<size_t>(m->part_lse - p.part);
+  }
+  m->launches += 1;
+  return timed(m, stream, [&] { return launch_fp4_rows(p, stream); });
 }
 
 // splits_out != nullptr: stop after the attention kernel and leave its split partials (part_o, part_lse) in the
@@ -696,6 +823,7 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
   if (!m->planned) return fail(GCT_ERR_INVALID, "attention: no plan (call gct_mgr_plan after the frame's append)");
   if (q_dev == nullptr || n_q <= 0 || n_q > m->cfg.tokens_per_frame)
     return fail(GCT_ERR_INVALID, "attention: n_q must be in [1, tokens_per_frame]");
+  if (m->fp4) return run_paged_fp4(m, block, q_dev, q_dtype, n_q, out_bf16, out_f32, lse_dev, stream, splits_out);
   const int H = m->cfg.num_heads;
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(q_dev);
   if (q_dtype == GCT_F32) {          // the reference casts q to the storage dtype (:419)
@@ -805,6 +933,33 @@ int gct_mgr_attention_exchange(gct_mgr_t* m, int block, const void* q_dev, int q
   // partial rows are laid out with n_q rows per split, which is what the exchange kernel indexes
   return launch_kv_exchange(m->part_o, m->part_lse, splits, static_cast<int>(rows), rank, world, epoch, recv_ptrs, out_ptrs,
                             flag_ptrs, slice_rows, m->status_dev, s);
+}
+
+int gct_mgr_read_frame_fp4(gct_mgr_t* m, int block, uint8_t* k_values_dev, void* k_scales_dev, uint8_t* v_values_dev, void* v_scales_dev, void* stream) {
+  uint8_t* const values[2] = {k_values_dev, v_values_dev};
+  void* const scales[2] = {k_scales_dev, v_scales_dev};
+  return mgr_read_frame_fp4(m, block, values, scales, static_cast<cudaStream_t>(stream));
+}
+
+int gct_mgr_read_page_fp4(gct_mgr_t* m, int block, int page, int rows, void* k_out_dev, void* v_out_dev, void* stream) {
+  int rc = check_bound(m);
+  if (rc != GCT_OK) return rc;
+  if (!m->fp4) return fail(GCT_ERR_INVALID, "gct_mgr_read_page_fp4: the cache is not held in 4 bits");
+  if (block < 0 || block >= m->cfg.num_blocks || page < 0 || page >= m->geo.max_num_pages || rows < 0 || rows > m->geo.page_size)
+    return fail(GCT_ERR_INVALID, "gct_mgr_read_page_fp4: page or rows out of range");
+  Fp4ReadLaunch p;
+  p.pool = m->pools4[block];
+  p.layout = m->fp4_page;
+  p.heads = m->cfg.num_heads;
+  p.tokens = rows;
+  p.num_pages = m->geo.max_num_pages;
+  p.page_rows = m->geo.page_size;
+  p.at.patch_page = page;
+  p.products[0] = static_cast<__nv_bfloat16*>(k_out_dev);
+  p.products[1] = static_cast<__nv_bfloat16*>(v_out_dev);
+  p.status = m->status_dev;
+  m->launches += 1;
+  return launch_fp4_read(p, static_cast<cudaStream_t>(stream));
 }
 
 int gct_mgr_device_status(gct_mgr_t* m, void* stream, int* status_out) {

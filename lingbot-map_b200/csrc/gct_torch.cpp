@@ -706,6 +706,127 @@ PyObject* py_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- 4-bit caches -------------------------------------------------------------------------------
+
+// (values, scales) of K, then of V, from `read`
+template <typename F>
+PyObject* fp4_rows(int64_t rows, int64_t heads, int64_t head_dim, const Tensor& like, F&& read) {
+  Tensor values[2], scales[2];
+  uint8_t* pv[2];
+  void* ps[2];
+  for (int i = 0; i < 2; ++i) {
+    values[i] = empty({rows, heads, head_dim}, at::kFloat8_e4m3fn, like);
+    scales[i] = empty({rows, heads, head_dim / 16}, at::kHalf, like);
+    pv[i] = static_cast<uint8_t*>(values[i].data_ptr());
+    ps[i] = scales[i].data_ptr();
+  }
+  check(unlocked([&] { return read(pv, ps); }));
+  PyObject* out = PyTuple_New(4);
+  if (out == nullptr) throw python_error();
+  for (int i = 0; i < 2; ++i) {
+    PyTuple_SET_ITEM(out, 2 * i, wrap(std::move(values[i])));
+    PyTuple_SET_ITEM(out, 2 * i + 1, wrap(std::move(scales[i])));
+  }
+  return out;
+}
+
+// read_frame_fp4(manager, device, block) -> (k_values, k_scales, v_values, v_scales)
+PyObject* py_read_frame_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need(n, 3, "read_frame_fp4");
+    gct_mgr_t* m = manager(a[0]);
+    const int block = static_cast<int>(integer(a[2]));
+    const c10::Device dev(c10::kCUDA, static_cast<c10::DeviceIndex>(integer(a[1])));
+    c10::cuda::CUDAGuard guard(dev);
+    const Tensor like = at::detail::empty_cuda({0}, at::kByte, dev, c10::nullopt);
+    const gct_mgr_config_t& cfg = gct::mgr_config(m);
+    return fp4_rows(cfg.tokens_per_frame, cfg.num_heads, kHeadDim, like,
+                    [&](uint8_t* const* v, void* const* s) { return gct_mgr_read_frame_fp4(m, block, v[0], s[0], v[1], s[1], stream_of(like)); });
+  });
+}
+
+// The caches [H, capacity / 128, bytes of a block] of one K and V pair.
+struct Fp4Cache {
+  const Tensor &k, &v;
+  int heads, head_dim, capacity;
+  Fp4Cache(PyObject* ok, PyObject* ov, int64_t dim) : k(tensor(ok, "cache_k")), v(tensor(ov, "cache_v")), head_dim(static_cast<int>(dim)) {
+    need_cuda(k, "cache_k");
+    if (k.scalar_type() != at::kByte || k.dim() != 3 || !k.is_contiguous() || k.size(2) != 128 * (dim / 2 + dim / 16) || v.scalar_type() != at::kByte ||
+        !v.is_contiguous() || v.sizes() != k.sizes() || v.device() != k.device())
+      value_error("4-bit caches must be contiguous uint8 [H, capacity / 128, 128 * (D / 2 + D / 16)] on one device");
+    heads = static_cast<int>(k.size(0));
+    capacity = static_cast<int>(128 * k.size(1));
+  }
+  uint8_t* kp() const { return static_cast<uint8_t*>(k.data_ptr()); }
+  uint8_t* vp() const { return static_cast<uint8_t*>(v.data_ptr()); }
+  Tensor rows(PyObject* o, const char* name) const {
+    const Tensor& t = tensor(o, name);
+    need_beside(t, name, k);
+    if (t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(1) != heads || t.size(2) != head_dim)
+      value_error(std::string(name) + " must be float32 [rows, " + std::to_string(heads) + ", " + std::to_string(head_dim) + "]");
+    return t.is_contiguous() ? t : t.contiguous();
+  }
+};
+// a row number or count (the library's are 32 bits)
+int row_number(PyObject* o, const char* name) {
+  const int64_t v = integer(o);
+  if (v < 0 || v > 0x7fffffff) value_error(std::string(name) + " is out of range");
+  return static_cast<int>(v);
+}
+
+// decode_attention_fp4(q, k_new, v_new, cache_k, cache_v, cached, store, workspace) -> out
+PyObject* py_decode_attention_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need(n, 8, "decode_attention_fp4");
+    const Tensor &q0 = tensor(a[0], "q"), &ws = tensor(a[7], "workspace");
+    if (q0.dim() != 3) value_error("q must be float32 [rows, H, D]");
+    const Fp4Cache c(a[3], a[4], q0.size(2));
+    const Tensor q = c.rows(a[0], "q"), k = c.rows(a[1], "k_new"), v = c.rows(a[2], "v_new");
+    if (k.size(0) != q.size(0) || v.size(0) != q.size(0)) value_error("decode attention: q, k and v must have the same number of rows");
+    need_beside(ws, "workspace", q);
+    const int cached = row_number(a[5], "cached"), store = PyObject_IsTrue(a[6]) == 1;
+    c10::cuda::CUDAGuard guard(q.device());
+    Tensor out = empty(q.sizes(), at::kFloat, q);
+    check(unlocked([&] {
+      return gct_decode_attention_fp4(q.data_ptr<float>(), k.data_ptr<float>(), v.data_ptr<float>(), static_cast<int>(q.size(0)), c.kp(), c.vp(), cached,
+                                      c.capacity, store, c.heads, c.head_dim, out.data_ptr<float>(), ws.data_ptr(), ws.nbytes(), stream_of(q));
+    }));
+    return wrap(std::move(out));
+  });
+}
+
+// decode_append_fp4(k, v, cache_k, cache_v, first)
+PyObject* py_decode_append_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need(n, 5, "decode_append_fp4");
+    const Tensor& k0 = tensor(a[0], "k");
+    if (k0.dim() != 3) value_error("k must be float32 [rows, H, D]");
+    const Fp4Cache c(a[2], a[3], k0.size(2));
+    const Tensor k = c.rows(a[0], "k"), v = c.rows(a[1], "v");
+    if (v.size(0) != k.size(0)) value_error("k and v must have the same number of rows");
+    const int first = row_number(a[4], "first");
+    c10::cuda::CUDAGuard guard(k.device());
+    check(unlocked([&] {
+      return gct_decode_append_fp4(k.data_ptr<float>(), v.data_ptr<float>(), static_cast<int>(k.size(0)), c.kp(), c.vp(), first, c.capacity, c.heads,
+                                   c.head_dim, stream_of(k));
+    }));
+    Py_RETURN_NONE;
+  });
+}
+
+// decode_read_fp4(cache_k, cache_v, head_dim, first, rows) -> (k_values, k_scales, v_values, v_scales)
+PyObject* py_decode_read_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need(n, 5, "decode_read_fp4");
+    const Fp4Cache c(a[0], a[1], integer(a[2]));
+    const int first = row_number(a[3], "first"), rows = row_number(a[4], "rows");
+    c10::cuda::CUDAGuard guard(c.k.device());
+    return fp4_rows(rows, c.heads, c.head_dim, c.k, [&](uint8_t* const* v, void* const* s) {
+      return gct_decode_read_fp4(c.kp(), c.vp(), first, rows, c.capacity, c.heads, c.head_dim, v[0], s[0], v[1], s[1], stream_of(c.k));
+    });
+  });
+}
+
 // rope3d_table(frame_index, pph, ppw, num_special, out)
 PyObject* py_rope3d_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -825,6 +946,10 @@ PyMethodDef g_methods[] = {FAST(prep_qkv),
                            FAST(evict),
                            FAST(rollback),
                            FAST(decode_attention),
+                           FAST(read_frame_fp4),
+                           FAST(decode_attention_fp4),
+                           FAST(decode_append_fp4),
+                           FAST(decode_read_fp4),
                            FAST(rope3d_table),
                            FAST(frustum_cull),
                            FAST(voxelize_frame),

@@ -13,14 +13,28 @@ import os
 _saved = {}
 
 
-def install(frame_attention: bool = True, patch_embed_attention: bool = None, camera_head: bool = None) -> None:
+def _bits_from_env(name: str, wide: int) -> int:
+    text = os.environ.get(name, str(wide))
+    if text not in (str(wide), "4"):
+        raise ValueError(f"{name} must be {wide} or 4, got {text!r}")
+    return int(text)
+
+
+def install(frame_attention: bool = True, patch_embed_attention: bool = None, camera_head: bool = None, kv_bits: int = None,
+            camera_kv_bits: int = None) -> None:
     """Rebind the reference's class names to the B200 implementations.  Call before building GCTStream.
 
     frame_attention: convert the aggregator's per-frame blocks.  patch_embed_attention: also convert the 24
     attention layers of the DINOv2 patch embed (vision_transformer.py:144-171; plain attention over 1004 tokens,
     no q/k norm, no RoPE); default from LINGBOT_B200_PATCH_EMBED (off unless set to 1).  camera_head: move the
     camera head's one-token-per-frame dict caches (heads/camera_head.py:284-358) onto the append-only device cache
-    of camera.py; default from LINGBOT_B200_CAMERA_HEAD (on unless set to 0)."""
+    of camera.py; default from LINGBOT_B200_CAMERA_HEAD (on unless set to 0).  kv_bits: 16 or 4, how the global blocks'
+    cache is held; default from LINGBOT_B200_KV_BITS (16).  camera_kv_bits: 32 or 4, the same for the camera head's
+    caches; default from LINGBOT_B200_CAMERA_KV_BITS (32)."""
+    kv_bits = _bits_from_env("LINGBOT_B200_KV_BITS", 16) if kv_bits is None else kv_bits
+    camera_kv_bits = _bits_from_env("LINGBOT_B200_CAMERA_KV_BITS", 32) if camera_kv_bits is None else camera_kv_bits
+    if kv_bits not in (16, 4) or camera_kv_bits not in (32, 4):
+        raise ValueError("kv_bits must be 16 or 4, camera_kv_bits 32 or 4")
     if patch_embed_attention is None:
         patch_embed_attention = os.environ.get("LINGBOT_B200_PATCH_EMBED", "0") == "1"
     if camera_head is None:
@@ -33,7 +47,7 @@ def install(frame_attention: bool = True, patch_embed_attention: bool = None, ca
     if not _saved:
         _saved.update(manager=cache_mod.FlashInferKVCacheManager, block=stream_mod.FlashInferBlock,
                       init=stream_mod.AggregatorStream.__init__)
-    cache_mod.FlashInferKVCacheManager = _manager_selector(_saved["manager"], B200KVCacheManager)
+    cache_mod.FlashInferKVCacheManager = _manager_selector(_saved["manager"], B200KVCacheManager, kv_bits)
     stream_mod.FlashInferBlock = B200Block
     if frame_attention:
         cls = stream_mod.AggregatorStream
@@ -46,6 +60,7 @@ def install(frame_attention: bool = True, patch_embed_attention: bool = None, ca
 
             cls.__init__ = wrapped_init
             cls._b200_wrapped = True
+    _saved["camera_kv_bits"] = camera_kv_bits
     if camera_head:
         import lingbot_map.heads.camera_head as head_mod
         hcls = head_mod.CameraCausalHead
@@ -56,13 +71,13 @@ def install(frame_attention: bool = True, patch_embed_attention: bool = None, ca
             def wrapped_head_init(self, *args, **kwargs):
                 head_init(self, *args, **kwargs)
                 from .camera import convert_camera_head
-                convert_camera_head(self)
+                convert_camera_head(self, _saved["camera_kv_bits"])
 
             hcls.__init__ = wrapped_head_init
             hcls._b200_wrapped = True
 
 
-def _manager_selector(reference_cls, b200_cls):
+def _manager_selector(reference_cls, b200_cls, kv_bits=16):
     """The class bound to the name `FlashInferKVCacheManager` while the backend is installed.  Constructing it gives
     a B200KVCacheManager, except with force_fp32=True (lingbot_map/aggregator/stream.py:227-228, set by
     gct_profile.py:293-296 for --dtype fp32): that is the reference's fp32 gather + SDPA comparison mode
@@ -77,7 +92,7 @@ def _manager_selector(reference_cls, b200_cls):
         def __new__(cls, *args, **kwargs):
             if kwargs.get("force_fp32", False):
                 return reference_cls(*args, **kwargs)
-            return b200_cls(*args, **kwargs)
+            return b200_cls(*args, **kwargs) if kv_bits == 16 else b200_cls(*args, kv_bits=kv_bits, **kwargs)
 
     FlashInferKVCacheManager.__doc__ = "selects B200KVCacheManager, or the reference's manager for force_fp32"
     return FlashInferKVCacheManager
