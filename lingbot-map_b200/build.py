@@ -7,7 +7,8 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["csrc/gct_attn_sm100.cu", "csrc/gct_elementwise.cu", "csrc/gct_manager.cu", "csrc/gct_static_scratch.cu",
-           "csrc/gct_exchange.cu", "csrc/gct_decode.cu", "csrc/gct_render.cu", "csrc/gct_fp4.cu"]
+           "csrc/gct_exchange.cu", "csrc/gct_decode.cu", "csrc/gct_render.cu", "csrc/gct_fp4.cu",
+           "csrc/gct_attn_fp4_sm100.cu"]
 HEADERS = ["csrc/gct_common.h", "csrc/gct_sm100.h", "csrc/gct_fp4.h", "../include/gct_b200.h"]
 LIB = os.path.join(HERE, "libgct_b200.so")
 BINDING_SOURCE = "csrc/gct_torch.cpp"

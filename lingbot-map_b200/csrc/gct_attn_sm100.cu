@@ -59,14 +59,12 @@ struct KernelArgs {
   float bounded_limit;
 };
 
-constexpr int kFfmaAhead = 4, kSumLag = 2;   // software pipeline of the exponential sweep, in pairs of logits
 // Register budget at two query tiles per CTA: 640 threads start with 96 registers each (61440 in total); the control
 // warpgroup shrinks to kControlRegs and the four softmax warpgroups grow to kSoftmaxRegs:
 // 128 * kControlRegs + 512 * kSoftmaxRegs <= 61440, both multiples of 8.
 constexpr int kControlRegs = 64;
 constexpr int kSoftmaxRegs = 104;      // 112 beside 32 was 2 % slower; of <2, true>'s 528 bytes of spill loads all but 76 go with the fallback
 static_assert(128 * kControlRegs + 512 * kSoftmaxRegs <= 61440, "register pool of the CTA exceeded");
-constexpr float kRescaleThreshold = 8.0f;   // in log2 units of the scaled logits
 
 // kCtas: CTAs that share an SM (one-tile kernels only), with shorter rings so that two fit.
 template <int QT, int kCtas>

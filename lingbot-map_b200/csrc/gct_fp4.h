@@ -151,6 +151,8 @@ struct Fp4RowsLaunch {
   int* status = nullptr;
 };
 int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream);
+// Attention of query tiles over a 4-bit pool; `a` as for launch_attention (tm_k, tm_v, key_norm_max and ctas_per_sm are not used).
+int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, cudaStream_t stream);
 // Key ranges that a call of `groups` x `heads` (head, eight queries) items over `blocks` blocks of 128 rows is cut into.
 int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters);
 

@@ -770,13 +770,18 @@ static int timed(gct_mgr* m, cudaStream_t stream, F&& launch) {
   }
   return rc;
 }
-static int timed_attention(gct_mgr* m, const AttnLaunch& a, cudaStream_t stream) {
-  return timed(m, stream, [&] { return launch_attention(a, stream); });
+static int timed_attention(gct_mgr* m, int block, const AttnLaunch& a, cudaStream_t stream) {
+  return timed(m, stream, [&] {
+    return m->fp4 ? launch_attention_fp4(a, m->pools4[block], m->fp4_page, m->geo.max_num_pages, stream) : launch_attention(a, stream);
+  });
 }
 
 extern "C" {
 
-// The same over a 4-bit cache; every result is final: splits_out != nullptr leaves it as the one partial result.
+// Query rows up to which a call over a 4-bit cache takes the kernel for few rows.
+static constexpr int kRowsMaxQueries = 16;
+
+// A few query rows over a 4-bit cache; every result is final: splits_out != nullptr leaves it as the one partial result.
 static int run_paged_fp4(gct_mgr* m, int block, const void* q_dev, int q_dtype, int n_q, __nv_bfloat16* out_bf16, float* out_f32, float* lse_dev,
                          cudaStream_t stream, int* splits_out) {
   if (q_dtype != GCT_F32 && q_dtype != GCT_BF16) return fail(GCT_ERR_INVALID, "attention: q dtype must be GCT_F32 or GCT_BF16");
@@ -823,7 +828,7 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
   if (!m->planned) return fail(GCT_ERR_INVALID, "attention: no plan (call gct_mgr_plan after the frame's append)");
   if (q_dev == nullptr || n_q <= 0 || n_q > m->cfg.tokens_per_frame)
     return fail(GCT_ERR_INVALID, "attention: n_q must be in [1, tokens_per_frame]");
-  if (m->fp4) return run_paged_fp4(m, block, q_dev, q_dtype, n_q, out_bf16, out_f32, lse_dev, stream, splits_out);
+  if (m->fp4 && n_q <= kRowsMaxQueries) return run_paged_fp4(m, block, q_dev, q_dtype, n_q, out_bf16, out_f32, lse_dev, stream, splits_out);
   const int H = m->cfg.num_heads;
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(q_dev);
   if (q_dtype == GCT_F32) {          // the reference casts q to the storage dtype (:419)
@@ -843,8 +848,10 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
   }
   AttnLaunch a;
   a.tm_q = m->tm_q;
-  a.tm_k = m->tm_k[block];
-  a.tm_v = m->tm_v[block];
+  if (!m->fp4) {
+    a.tm_k = m->tm_k[block];
+    a.tm_v = m->tm_v[block];
+  }
   a.page_table = m->table_dev;
   a.n_pages = m->plan_pages;
   a.page_len = m->geo.page_size;
@@ -863,7 +870,7 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
   const int64_t rows = static_cast<int64_t>(n_q) * H;
   // Bounded mode: every key of this block's cache went through the manager, so |q_row| * max|k| bounds the row's
   // logits; while that bound stays small it replaces the running row maximum (decided per CTA inside the kernel).
-  if (m->bounded_enabled && m->key_norm_max != nullptr && m->key_norm_valid[block] && a.q_tiles_per_cta == 2) {
+  if (m->bounded_enabled && m->key_norm_max != nullptr && m->key_norm_valid[block] && a.q_tiles_per_cta == 2 && !m->fp4) {
     a.key_norm_max = m->key_norm_max + static_cast<size_t>(block) * H;
     a.bounded_limit = kBoundedLimit;
   }
@@ -873,19 +880,19 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
     a.part_lse = m->part_lse;
     *splits_out = a.splits;
     m->launches += 1;
-    return timed_attention(m, a, stream);
+    return timed_attention(m, block, a, stream);
   }
   if (a.splits == 1 && out_bf16 != nullptr && lse_dev == nullptr) {
     a.final_bf16 = true;
     a.out = out_bf16;
     m->launches += 1;
-    return timed_attention(m, a, stream);
+    return timed_attention(m, block, a, stream);
   }
   a.final_bf16 = false;
   a.part_o = m->part_o;
   a.part_lse = m->part_lse;
   // partial rows are laid out with n_q rows per split
-  rc = timed_attention(m, a, stream);
+  rc = timed_attention(m, block, a, stream);
   if (rc != GCT_OK) return rc;
   m->launches += 2;
   return launch_merge(m->part_o, m->part_lse, a.splits, rows, out_bf16, out_f32, lse_dev, stream);

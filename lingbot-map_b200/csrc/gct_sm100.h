@@ -236,5 +236,8 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return r;
 }
 
+constexpr int kFfmaAhead = 4, kSumLag = 2;   // software pipeline of the exponential sweep, in pairs of logits
+constexpr float kRescaleThreshold = 8.0f;    // growth of a row's maximum that moves the running reference, in log2 units of the scaled logits
+
 }  // namespace
 }  // namespace gct
