@@ -13,6 +13,7 @@
 // [2^14, 2^15) - bf16 queries lose nothing that an fp32 sum would keep - and the row's factor goes back into the multiply-add in front
 // of its exponential.  Weights are half-precision numbers of up to 2^15: eleven bits where bf16 has eight.
 #include <mutex>
+#include <type_traits>
 
 #include "gct_fp4.h"
 #include "gct_sm100.h"
@@ -22,7 +23,8 @@ namespace {
 
 constexpr int kPackedStages = 6, kTileStages = 4;          // packed blocks in flight; unpacked tiles (K, V, K, V)
 constexpr uint32_t kPackedBytes = kFp4BlockBytes<64>;
-constexpr float kFp4Shift = 7.f;                           // weights are at most 2^(kRescaleThreshold + kFp4Shift)
+constexpr float kFp4Shift = 7.f;                           // running maximum: weights are at most 2^(kRescaleThreshold + kFp4Shift)
+constexpr float kFixedShift = 15.f;                        // fixed reference: weights are at most 2^15
 // half-precision operands: formats 0; K-major A and B for S, MN-major B for P V
 constexpr uint32_t kIdescS16 = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescPV16 = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
@@ -41,9 +43,10 @@ struct Fp4Smem {
   static constexpr uint32_t packed_off = tile_off + kTileStages * kTileBytes;
   static constexpr uint32_t pair_off = packed_off + kPackedStages * kPackedBytes;      // [2][QT][2][128] floats, as in gct_attn_kernel
   static constexpr uint32_t factor_off = pair_off + 2 * QT * 2 * 128 * 4;              // [QT][128] floats: a row's multiplier in front of exp2
-  static constexpr uint32_t bar_off = factor_off + QT * 128 * 4;
-  // q_full, q_ready, packed_full/empty[6], tile_full/empty[4], per query tile s_full, s_empty, p_full[2], pv_full
-  static constexpr int n_bars = 2 + 2 * kPackedStages + 2 * kTileStages + 5 * QT;
+  static constexpr uint32_t ref_off = factor_off + QT * 128 * 4;                       // [QT][128] floats: a row's fixed reference
+  static constexpr uint32_t bar_off = ref_off + QT * 128 * 4;
+  // q_full, q_ready, verdict, packed_full/empty[6], tile_full/empty[4], per query tile s_full, s_empty, p_full[2], pv_full[2]
+  static constexpr int n_bars = 3 + 2 * kPackedStages + 2 * kTileStages + 6 * QT;
   static constexpr uint32_t misc_off = bar_off + n_bars * 8;
   static constexpr uint32_t total = misc_off + 16;
 };
@@ -58,6 +61,8 @@ struct Fp4Args {
   __nv_bfloat16* out;
   float *part_o, *part_lse;
   int* status;
+  const float* key_norm_max;      // [heads]: bounds the 2-norm of every key of a head (null: unknown)
+  float fixed_limit;              // largest bound of a row's exponents that the fixed reference is tried with
 };
 
 template <int QT>
@@ -69,17 +74,20 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   const uint32_t bars = sbase + L::bar_off;
   auto bar_q_full = [&]() { return bars; };
   auto bar_q_ready = [&]() { return bars + 8u; };
-  auto bar_packed_full = [&](int s) { return bars + 8u * (2 + s); };
-  auto bar_packed_empty = [&](int s) { return bars + 8u * (2 + kPackedStages + s); };
-  auto bar_tile_full = [&](int s) { return bars + 8u * (2 + 2 * kPackedStages + s); };
-  auto bar_tile_empty = [&](int s) { return bars + 8u * (2 + 2 * kPackedStages + kTileStages + s); };
-  constexpr int kFirst = 2 + 2 * kPackedStages + 2 * kTileStages;
-  auto bar_s_full = [&](int t) { return bars + 8u * (kFirst + 5 * t + 0); };
-  auto bar_s_empty = [&](int t) { return bars + 8u * (kFirst + 5 * t + 1); };
-  auto bar_p_full = [&](int t, int half) { return bars + 8u * (kFirst + 5 * t + 2 + half); };
-  auto bar_pv_full = [&](int t) { return bars + 8u * (kFirst + 5 * t + 4); };
+  auto bar_verdict = [&]() { return bars + 16u; };
+  auto bar_packed_full = [&](int s) { return bars + 8u * (3 + s); };
+  auto bar_packed_empty = [&](int s) { return bars + 8u * (3 + kPackedStages + s); };
+  auto bar_tile_full = [&](int s) { return bars + 8u * (3 + 2 * kPackedStages + s); };
+  auto bar_tile_empty = [&](int s) { return bars + 8u * (3 + 2 * kPackedStages + kTileStages + s); };
+  constexpr int kFirst = 3 + 2 * kPackedStages + 2 * kTileStages;
+  auto bar_s_full = [&](int t) { return bars + 8u * (kFirst + 6 * t + 0); };
+  auto bar_s_empty = [&](int t) { return bars + 8u * (kFirst + 6 * t + 1); };
+  auto bar_p_full = [&](int t, int half) { return bars + 8u * (kFirst + 6 * t + 2 + half); };
+  auto bar_pv_full = [&](int t, int half) { return bars + 8u * (kFirst + 6 * t + 4 + half); };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::misc_off);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(smem + L::misc_off + 4);
+  volatile int* cta_exact = reinterpret_cast<volatile int*>(smem + L::misc_off + 8);      // running maximum from the start
+  volatile int* cta_redo = reinterpret_cast<volatile int*>(smem + L::misc_off + 12);      // the fixed reference has not held
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kProducerWarp = 8 * QT, kFirstMmaWarp = 8 * QT + 1, kFirstUnpackWarp = 8 * QT + 4;
@@ -108,6 +116,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   if (threadIdx.x == 0) {
     mbar_init(bar_q_full(), 1);
     mbar_init(bar_q_ready(), 4 * QT);
+    mbar_init(bar_verdict(), 8 * QT);
     for (int s = 0; s < kPackedStages; ++s) {
       mbar_init(bar_packed_full(s), 1);
       mbar_init(bar_packed_empty(s), 4);
@@ -121,9 +130,12 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       mbar_init(bar_s_empty(t), 8);
       mbar_init(bar_p_full(t, 0), 4);
       mbar_init(bar_p_full(t, 1), 4);
-      mbar_init(bar_pv_full(t), 1);
+      mbar_init(bar_pv_full(t, 0), 1);
+      mbar_init(bar_pv_full(t, 1), 1);
     }
     *cta_abort = 0;
+    *cta_exact = a.key_norm_max == nullptr;
+    *cta_redo = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kFirstMmaWarp) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
@@ -133,6 +145,10 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
+
+  // A CTA goes through its KV range a second time when the fixed reference has not held; every role but the softmax waits here for
+  // the verdict: behind the first pass, or as soon as the running maximum is chosen from the start (a short range may be unpacked before that).
+  auto again = [&]() -> bool { return mbar_wait(bar_verdict(), 0, cta_abort, a.status) && *cta_redo != 0; };
 
   // Valid rows of block g; `rows`: rows that the block holds in memory.
   auto block_rows = [&](int g, int& page_index, int& block, int& rows) -> int {
@@ -146,9 +162,9 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     // =========================== dequantising warps ===========================
     if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4UnpackRegs));
     const int tid = threadIdx.x - 32 * kFirstUnpackWarp;
-    for (int i = 0; i < 2 * nblk; ++i) {
+    for (int i = 0, end = 2 * nblk; i < end || (i == 2 * nblk && again() && (end = 4 * nblk)); ++i) {
       int pi, block, rows;
-      const int valid = block_rows(g0 + (i >> 1), pi, block, rows);
+      const int valid = block_rows(g0 + (i >> 1) - (i >= 2 * nblk ? nblk : 0), pi, block, rows);
       const int ps = i % kPackedStages, ts = i % kTileStages;
       if (!__all_sync(0xffffffffu, mbar_wait(bar_packed_full(ps), (i / kPackedStages) & 1, cta_abort, a.status) &&
                                        mbar_wait(bar_tile_empty(ts), ((i / kTileStages) & 1) ^ 1u, cta_abort, a.status)))
@@ -190,9 +206,9 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       for (int t = 0; t < QT; ++t) tma_load_4d(sbase + L::q_off + t * kTileBytes, &tm_q, bar_q_full(), 0, h, (qg * QT + t) * kTileM, 0);
       int cur = -1;
       const uint8_t* base = nullptr;
-      for (int i = 0; i < 2 * nblk; ++i) {
+      for (int i = 0, end = 2 * nblk; i < end || (i == 2 * nblk && again() && (end = 4 * nblk)); ++i) {
         int pi, block, rows;
-        block_rows(g0 + (i >> 1), pi, block, rows);
+        block_rows(g0 + (i >> 1) - (i >= 2 * nblk ? nblk : 0), pi, block, rows);
         if (pi != cur) {
           const int page = __ldg(a.page_table + pi);
           cur = pi;
@@ -226,38 +242,48 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_ss(lead, tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS16, k > 0);
       };
-      auto issue_pv = [&](int s, uint32_t accumulate) {
+      auto issue_pv = [&](int s, int half, uint32_t accumulate) {
         const uint64_t bd = smem_desc(sbase + L::tile_off + s * kTileBytes, 16, 1024);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 4 * half; k < 4 * half + 4; ++k)
           umma_ts(lead, tmem_base + kOCol + t * 64, tmem_base + kPCol + t * 64 + k * 8, bd + k * 128, kIdescPV16, k > 0 ? 1u : accumulate);
       };
       auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, a.status)); };
-      bool ok = wait(bar_q_ready(), 0) && wait(bar_tile_full(k_stage(0)), 0);
-      if (ok) {
+      // block j of all passes; S_j may overwrite S_{j-1} once that is in registers
+      auto start_s = [&](int j) -> bool {
+        const int s = k_stage(j);
+        if (j > 0 && !wait(bar_s_empty(t), (j - 1) & 1)) return false;
+        if (!wait(bar_tile_full(s), tile_parity(j))) return false;
         tc_fence_after();
-        issue_s(k_stage(0));
+        issue_s(s);
         tc_commit_elected(lead, bar_s_full(t));
-        tc_commit_elected(lead, bar_tile_empty(k_stage(0)));
-      }
-      for (int j = 0; ok && j < nblk; ++j) {
-        if (j + 1 < nblk) {
-          const int s = k_stage(j + 1);
-          if (!(ok = wait(bar_s_empty(t), j & 1))) break;
-          if (!(ok = wait(bar_tile_full(s), tile_parity(j + 1)))) break;
+        tc_commit_elected(lead, bar_tile_empty(s));
+        return true;
+      };
+      bool ok = wait(bar_q_ready(), 0);
+      bool both = *cta_exact != 0;            // a running maximum: either half's threads may have rescaled O before
+      for (int first = 0; ok;) {
+        ok = start_s(first);
+        for (int j = first; ok && j < first + nblk; ++j) {
+          if (j + 1 < first + nblk && !(ok = start_s(j + 1))) break;
+          const int s = v_stage(j);
+          if (!(ok = wait(bar_p_full(t, 0), j & 1))) break;
+          if (both && !(ok = wait(bar_p_full(t, 1), j & 1))) break;
+          if (!(ok = wait(bar_tile_full(s), tile_parity(j)))) break;
           tc_fence_after();
-          issue_s(s);
-          tc_commit_elected(lead, bar_s_full(t));
+          issue_pv(s, 0, j > first ? 1u : 0u);
+          tc_commit_elected(lead, bar_pv_full(t, 0));
+          if (!both) {
+            if (!(ok = wait(bar_p_full(t, 1), j & 1))) break;
+            tc_fence_after();
+          }
+          issue_pv(s, 1, 1u);
+          tc_commit_elected(lead, bar_pv_full(t, 1));
           tc_commit_elected(lead, bar_tile_empty(s));
         }
-        const int s = v_stage(j);
-        if (!(ok = wait(bar_p_full(t, 0), j & 1))) break;
-        if (!(ok = wait(bar_p_full(t, 1), j & 1))) break;
-        if (!(ok = wait(bar_tile_full(s), tile_parity(j)))) break;
-        tc_fence_after();
-        issue_pv(s, j > 0 ? 1u : 0u);
-        tc_commit_elected(lead, bar_pv_full(t));
-        tc_commit_elected(lead, bar_tile_empty(s));
+        if (!ok || both || first > 0 || !__all_sync(0xffffffffu, again())) break;
+        first = nblk;
+        both = true;
       }
     }
   } else {
@@ -286,8 +312,9 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     };
     constexpr uint32_t kPairSlot = QT * 2 * 128 * 4;
 
-    // ---- once per CTA: the Q row in half precision ----
+    // ---- once per CTA: the Q row in half precision, its factor and its fixed reference ----
     float* factor = reinterpret_cast<float*>(smem + L::factor_off) + t * 128 + row;
+    float* reference = reinterpret_cast<float*>(smem + L::ref_off) + t * 128 + row;
     if (half == 0) {
       ok = wait_v(bar_q_full(), 0);
       if (ok) {
@@ -302,76 +329,66 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
         }
         // at most 2^126; 1 for a row of zeros or with a value that is not finite
         const int up = top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
-        const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-        *factor = a.scale_log2 / f;
+        const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23), c = a.scale_log2 / f;
+        *factor = c;
+        float sq = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[4 * j + i] = pack_f16x2(__uint_as_float(w[4 * j + i] << 16) * f, __uint_as_float(w[4 * j + i] & 0xffff0000u) * f);
+          for (int i = 0; i < 4; ++i) {
+            w[4 * j + i] = pack_f16x2(__uint_as_float(w[4 * j + i] << 16) * f, __uint_as_float(w[4 * j + i] & 0xffff0000u) * f);
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[4 * j + i]));
+            sq = fmaf(x.x, x.x, fmaf(x.y, x.y, sq));
+          }
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_row + ((static_cast<uint32_t>(j) ^ (row & 7)) << 4)), "r"(w[4 * j]),
                        "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                        : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_q_ready());
+        if (a.key_norm_max != nullptr) {
+          const float ref = sqrtf(sq) * __ldg(a.key_norm_max + h) * c;
+          *reference = ref;
+          if (!(ref <= a.fixed_limit)) *cta_exact = 1;     // too loose, infinite or NaN
+        }
       }
     }
-    pair_sync();                                           // both warps of the row, also after a failed wait
+    auto softmax_sync = [&]() { asm volatile("bar.sync 15, %0;" ::"n"(256 * QT) : "memory"); };      // all softmax threads, also after a failed wait
+    softmax_sync();
+    const bool fixed = *cta_exact == 0;
+    if (lane == 0) {
+      if (half == 0 && ok) mbar_arrive(bar_q_ready());
+      if (!fixed) mbar_arrive(bar_verdict());
+    }
     const float c = *factor;
     float m = -INFINITY, l = 0.f;                          // m: reference maximum (units of S); l: sum over this half
 
-    int pi = g0 / a.blocks_per_page;
+    int pi, left;
     auto blocks_of = [&](int page) { return page == a.n_pages - 1 ? a.total_blocks - page * a.blocks_per_page : a.blocks_per_page; };
-    int left = blocks_of(pi) - (g0 - pi * a.blocks_per_page);
+    auto rewind = [&]() {
+      pi = g0 / a.blocks_per_page;
+      left = blocks_of(pi) - (g0 - pi * a.blocks_per_page);
+    };
     auto tail_valid = [&]() -> int {
       const int valid = (pi == a.n_pages - 1 ? a.last_page_len : a.page_len) - (blocks_of(pi) - 1) * kBlockN - 64 * half;
       left = blocks_of(++pi);
       return valid;
     };
-    int met = 0;
-    for (int j = 0; ok && j < nblk; ++j) {
-      if (!(ok = wait_u(bar_s_full(t), j & 1))) break;
-      tc_fence_after();
-      uint32_t s[64], pk[32];
-      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      mbar_arrive_elected(lead, bar_s_empty(t));
-      if (--left == 0) {
-        const int valid = tail_valid();
-        if (valid < 64) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= valid) s[i] = 0xff800000u;
-        }
-      }
-      float mxc[4];
-#pragma unroll
-      for (int ch = 0; ch < 4; ++ch) mxc[ch] = __uint_as_float(s[ch]);
-#pragma unroll
-      for (int i = 4; i < 64; i += 2) mxc[(i >> 1) & 3] = max3(mxc[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-      float mx = fmaxf(fmaxf(mxc[0], mxc[1]), fmaxf(mxc[2], mxc[3]));
-      mx = fmaxf(mx, pair_exchange(mx, (j & 1) * kPairSlot));
-      ++met;
-      float alpha = 1.f;
-      if ((mx - m) * c > kRescaleThreshold) {              // always true on the first block (m = -inf)
-        alpha = fast_exp2((m - mx) * c);
-        m = mx;
-      }
-      const float2 c2 = make_float2(c, c), nmc2 = make_float2(kFp4Shift - m * c, kFp4Shift - m * c);
+    // P = exp2(S c + shift) of 64 logits as half-precision pairs, and their sum, software-pipelined over pairs as in gct_attn_kernel.  kNum of
+    // kDen pairs take the FMA pipe; kBelow: exponents may lie below -126.
+    auto sweep = [&](uint32_t (&s)[64], uint32_t (&pk)[32], float shift, auto below, auto num, auto den) -> float {
+      constexpr bool kBelow = decltype(below)::value;
+      constexpr int kNum = decltype(num)::value, kDen = decltype(den)::value;
+      const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
       float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
       auto pair_ffma = [&](int q) {
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), c2, nmc2);
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), c2, shift2);
         s[2 * q] = __float_as_uint(x.x);
         s[2 * q + 1] = __float_as_uint(x.y);
       };
       auto pair_exp = [&](int q) {
-        constexpr int kNum = QT == 2 ? 2 : 1, kDen = QT == 2 ? 7 : 3;      // pairs on the FMA pipe, as in gct_attn_kernel
         if (((q + 1) * kNum) / kDen != (q * kNum) / kDen) {
-          const float2 e = exp2_poly2(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])));
+          const float2 x = make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
+          const float2 e = kBelow ? exp2_poly2(x) : exp2_poly2_inrange(x);
           s[2 * q] = __float_as_uint(e.x);
           s[2 * q + 1] = __float_as_uint(e.y);
         } else {
@@ -394,34 +411,129 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       }
 #pragma unroll
       for (int q = 32 - kSumLag; q < 32; ++q) pair_sum(q);
-      l = fmaf(l, alpha, (acc0.x + acc0.y) + (acc1.x + acc1.y));
-      if (j > 0) {
-        if (!(ok = wait_u(bar_pv_full(t), (j - 1) & 1))) break;
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-          uint32_t ob[32];
-          tmem_ld32(o_addr, ob);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * alpha);
-          tmem_st32(o_addr, ob);
-        }
-      }
+      return (acc0.x + acc0.y) + (acc1.x + acc1.y);
+    };
+    using std::integral_constant;
+    using Yes = std::true_type;
+    using No = std::false_type;
+    // S of block j in registers, the tile free for the next
+    auto load_s = [&](int j, uint32_t (&s)[64]) -> bool {
+      if (!wait_u(bar_s_full(t), j & 1)) return false;
+      tc_fence_after();
+      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      mbar_arrive_elected(lead, bar_s_empty(t));
+      return true;
+    };
+    auto store_p = [&](const uint32_t (&pk)[32]) {
       tmem_st32(p_addr, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       mbar_arrive_elected(lead, bar_p_full(t, half));
+    };
+    auto mask = [&](uint32_t (&s)[64], int valid) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (i >= valid) s[i] = 0xff800000u;
+    };
+
+    // ---- fixed reference: |q| max|k| bounds every exponent of the row (Cauchy-Schwarz); no maximum, no exchange, no rescaling ----
+    // Weights are exp2(x - ref + 15), at most 2^15.  Half precision holds them to 2^-25 at least, so over n keys at most n 2^-25 of the sum is lost
+    // to rounding small ones; a row whose sum is at least n 2^-15 has lost less than 2^-10 of it.  A CTA with a row below that goes through its
+    // range again with the running maximum.
+    bool held = false;
+    rewind();
+    if (fixed) {
+      const float shift = kFixedShift - *reference;
+      int keys = nblk * kBlockN;
+      for (int j = 0; ok && j < nblk; ++j) {
+        uint32_t s[64], pk[32];
+        if (!(ok = load_s(j, s))) break;
+        int valid = 64;
+        if (--left == 0) {
+          valid = tail_valid();
+          keys -= kBlockN - min(valid + 64 * half, kBlockN);
+        }
+        if (valid < 64) {
+          mask(s, valid);
+          l += sweep(s, pk, shift, Yes(), integral_constant<int, 0>(), integral_constant<int, 1>());
+        } else {
+          l += sweep(s, pk, shift, No(), integral_constant<int, 2>(), integral_constant<int, 5>());
+        }
+        if (j > 0) {
+          if (!(ok = wait_u(bar_pv_full(t, half), (j - 1) & 1))) break;
+          tc_fence_after();
+        }
+        store_p(pk);
+      }
+      __syncwarp();
+      if (ok && nblk > 0) ok = wait_v(bar_pv_full(t, 1), (nblk - 1) & 1);
+      const float other = pair_exchange(l, 0);
+      l = half == 0 ? l + other : other + l;
+      if (ok && !(l >= static_cast<float>(keys) * 0x1p-15f)) *cta_redo = 1;
+      softmax_sync();
+      held = *cta_redo == 0;
+      if (lane == 0) mbar_arrive(bar_verdict());
+      if (held) {
+        m = *reference;
+      } else {
+        l = 0.f;
+        rewind();
+      }
     }
-    __syncwarp();
-    for (; met < nblk; ++met) pair_sync();
+    // ---- running maximum ----
+    if (!held) {
+      const int first = fixed ? nblk : 0;
+      int met = 0;
+      for (int j = first; ok && j < first + nblk; ++j) {
+        uint32_t s[64], pk[32];
+        if (!(ok = load_s(j, s))) break;
+        if (--left == 0) {
+          const int valid = tail_valid();
+          if (valid < 64) mask(s, valid);
+        }
+        float mxc[4];
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) mxc[ch] = __uint_as_float(s[ch]);
+#pragma unroll
+        for (int i = 4; i < 64; i += 2) mxc[(i >> 1) & 3] = max3(mxc[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        float mx = fmaxf(fmaxf(mxc[0], mxc[1]), fmaxf(mxc[2], mxc[3]));
+        mx = fmaxf(mx, pair_exchange(mx, ((met + 1) & 1) * kPairSlot));
+        ++met;
+        float alpha = 1.f;
+        if ((mx - m) * c > kRescaleThreshold) {            // always true on the first block (m = -inf)
+          alpha = fast_exp2((m - mx) * c);
+          m = mx;
+        }
+        const float sum = sweep(s, pk, kFp4Shift - m * c, Yes(), integral_constant<int, QT == 2 ? 2 : 1>(), integral_constant<int, QT == 2 ? 7 : 3>());
+        l = fmaf(l, alpha, sum);
+        if (j > first) {
+          if (!(ok = wait_u(bar_pv_full(t, 1), (j - 1) & 1))) break;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+            uint32_t ob[32];
+            tmem_ld32(o_addr, ob);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * alpha);
+            tmem_st32(o_addr, ob);
+          }
+        }
+        store_p(pk);
+      }
+      __syncwarp();
+      for (; met < nblk; ++met) pair_sync();
+      if (ok && nblk > 0) ok = wait_v(bar_pv_full(t, 1), (first + nblk - 1) & 1);
+      const float other = pair_exchange(l, ((nblk + 1) & 1) * kPairSlot);
+      l = half == 0 ? l + other : other + l;
+      m = m * c + (kFixedShift - kFp4Shift);               // as below: the exponent that weighs 2^kFixedShift
+    }
 
     // ---- epilogue: O / l ----
-    if (ok && nblk > 0) ok = wait_v(bar_pv_full(t), (nblk - 1) & 1);
-    {
-      const float other = pair_exchange(l, (nblk & 1) * kPairSlot);
-      l = half == 0 ? l + other : other + l;
-    }
     const int qrow = (qg * QT + t) * kTileM + row;
     if (ok && nblk > 0) {
       tc_fence_after();
@@ -449,7 +561,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           for (int q4 = 0; q4 < 8; ++q4)
             dst[q4] = make_float4(__uint_as_float(ob[q4 * 4 + 0]) * inv, __uint_as_float(ob[q4 * 4 + 1]) * inv, __uint_as_float(ob[q4 * 4 + 2]) * inv,
                                   __uint_as_float(ob[q4 * 4 + 3]) * inv);
-          if (half == 0) a.part_lse[prow] = (m * c + log2f(l) - kFp4Shift) * 0.6931471805599453f;
+          if (half == 0) a.part_lse[prow] = (m + log2f(l) - kFixedShift) * 0.6931471805599453f;
         }
       }
     }
@@ -517,6 +629,8 @@ int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layo
   k.part_o = a.part_o;
   k.part_lse = a.part_lse;
   k.status = a.status;
+  k.key_norm_max = a.key_norm_max;
+  k.fixed_limit = a.bounded_limit;
   if (a.splits < 1 || a.splits > k.total_blocks) return fail(GCT_ERR_INVALID, "attention: splits out of range");
   if (a.split_len != 0) {
     const long long rest = static_cast<long long>(k.total_blocks) - static_cast<long long>(a.splits - 1) * a.split_len;

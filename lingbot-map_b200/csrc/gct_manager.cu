@@ -135,6 +135,8 @@ static constexpr int kRowsCounters = 4096;     // (head, eight queries) items of
 // Largest |q| * max|k| * scale * log2(e) for which the bound may stand in for the row maximum: all exponents stay
 // in [-2 * limit, 0], far inside the fp32 / bf16 exponent range.
 static constexpr float kBoundedLimit = 40.0f;
+// The same for a 4-bit cache, whose kernel checks afterwards that the reference was not too far above a row's logits and repeats where it was.
+static constexpr float kFp4BoundedLimit = 30.0f;
 
 static void reset_block(const gct_mgr* m, BlockState& b) {
   b.scale_pages.clear();
@@ -870,9 +872,9 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
   const int64_t rows = static_cast<int64_t>(n_q) * H;
   // Bounded mode: every key of this block's cache went through the manager, so |q_row| * max|k| bounds the row's
   // logits; while that bound stays small it replaces the running row maximum (decided per CTA inside the kernel).
-  if (m->bounded_enabled && m->key_norm_max != nullptr && m->key_norm_valid[block] && a.q_tiles_per_cta == 2 && !m->fp4) {
+  if (m->bounded_enabled && m->key_norm_max != nullptr && m->key_norm_valid[block] && (a.q_tiles_per_cta == 2 || m->fp4)) {
     a.key_norm_max = m->key_norm_max + static_cast<size_t>(block) * H;
-    a.bounded_limit = kBoundedLimit;
+    a.bounded_limit = m->fp4 ? kFp4BoundedLimit : kBoundedLimit;
   }
   if (splits_out != nullptr) {
     a.final_bf16 = false;

@@ -272,6 +272,45 @@ def test_many_query_rows(patches, H, frames, n_q):
     assert m.device_status() == 0
 
 
+@pytest.mark.parametrize("patches,n_q", [(122, 128), (300, 306), (300, 40)])
+@pytest.mark.parametrize("regime", ["fixed", "off", "too large", "repeated", "some rows repeated"])
+def test_softmax_reference(patches, n_q, regime):
+    """The fixed reference |q| max|k|, the running maximum it gives way to, and the second pass of a CTA in which a row turned out to lie far
+    below its reference: keys that all point against the queries."""
+    T, H = patches + NS, 2
+    rs = np.random.RandomState(patches)
+    m = manager(T, H, scale=1, window=2, total=40)
+    against = regime.endswith("repeated")
+    u = np.where(rs.standard_normal(64) > 0, 1.0, -1.0)
+    for t in range(5):
+        k = rs.standard_normal((T, H, 64)) * (0.05 if against else 1.0) - (u if against else 0.0)
+        m.append_frame(0, dev(k, torch.bfloat16), dev(rs.standard_normal((T, H, 64)), torch.bfloat16))
+        m.evict_frames(0, 1, 2)
+    q = rs.standard_normal((n_q, H, 64)) * (8.0 if regime == "too large" else 1.0)
+    if against:
+        rows = slice(None) if regime == "repeated" else slice(n_q // 2, n_q // 2 + 3)
+        q[rows] = 2.2 * u + 0.1 * q[rows]                 # logits of about -18 (26 in base 2), the reference 29
+    q = bf(q)
+    k, v = (host(x) for x in m._gather_kv(0))
+    norms = m.key_norm_max.double().cpu().numpy()[0]
+    true_norms = np.sqrt((k ** 2).sum(-1)).max(0)
+    assert (norms >= true_norms).all() and (norms <= true_norms * 1.3).all()          # evicted frames had norms of about the same
+    reference = np.sqrt((q ** 2).sum(-1)) * norms / 8 * 1.4427
+    assert (reference.max() > 30) == (regime == "too large")
+    if regime == "off":
+        m.set_bounded_mode(False)
+    want, want_lse, weighted = F.attention(q, k, v)
+    out, lse = m.compute_attention(0, dev(q, torch.bfloat16), return_lse=True)
+    tol = bound_frame(len(k), spread_of(q, k), weighted, want)
+    assert (np.abs(host(out) - want) <= tol).all(), float((np.abs(host(out) - want) / tol).max())
+    assert np.abs(host(lse) - want_lse).max() <= 2.0 ** -16 * spread_of(q, k) + 2.0 ** -13 + len(k) * 2.0 ** -23
+    assert m.device_status() == 0
+    # the norms found again from the pool alone
+    m.rescan_key_norms()
+    again = m.key_norm_max.double().cpu().numpy()[0]
+    assert (again >= true_norms).all() and (again <= norms * 1.001).all()
+
+
 # ---------------------------------------------------------------- the camera head's caches
 def decode_bound(keys, spread, weighted):
     """fp32 results: as bound_rows without the last rounding; the rounding of the division and of the result, 2^-23, is inside the first terms."""
