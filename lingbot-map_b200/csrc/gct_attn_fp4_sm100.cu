@@ -21,7 +21,7 @@
 namespace gct {
 namespace {
 
-constexpr int kPackedStages = 6, kTileStages = 4;          // packed blocks in flight; unpacked tiles (K, V, K, V)
+constexpr int kPackedStages = 4, kTileStages = 2;          // blocks (K and V) in flight packed, and unpacked
 constexpr uint32_t kPackedBytes = kFp4BlockBytes<64>;
 constexpr float kFp4Shift = 7.f;                           // running maximum: weights are at most 2^(kRescaleThreshold + kFp4Shift)
 constexpr float kFixedShift = 15.f;                        // fixed reference: weights are at most 2^15
@@ -40,13 +40,13 @@ template <int QT>
 struct Fp4Smem {
   static constexpr uint32_t q_off = 0;
   static constexpr uint32_t tile_off = q_off + QT * kTileBytes;
-  static constexpr uint32_t packed_off = tile_off + kTileStages * kTileBytes;
-  static constexpr uint32_t pair_off = packed_off + kPackedStages * kPackedBytes;      // [2][QT][2][128] floats, as in gct_attn_kernel
+  static constexpr uint32_t packed_off = tile_off + kTileStages * 2 * kTileBytes;
+  static constexpr uint32_t pair_off = packed_off + kPackedStages * 2 * kPackedBytes;      // [2][QT][2][128] floats, as in gct_attn_kernel
   static constexpr uint32_t factor_off = pair_off + 2 * QT * 2 * 128 * 4;              // [QT][128] floats: a row's multiplier in front of exp2
   static constexpr uint32_t ref_off = factor_off + QT * 128 * 4;                       // [QT][128] floats: a row's fixed reference
   static constexpr uint32_t bar_off = ref_off + QT * 128 * 4;
-  // q_full, q_ready, verdict, packed_full/empty[6], tile_full/empty[4], per query tile s_full, s_empty, p_full[2], pv_full[2]
-  static constexpr int n_bars = 3 + 2 * kPackedStages + 2 * kTileStages + 6 * QT;
+  // q_full, q_ready, verdict, packed_full/empty[], K and V tile_full/empty[], per query tile s_full, s_empty, p_full[2], pv_full[2]
+  static constexpr int n_bars = 3 + 2 * kPackedStages + 4 * kTileStages + 6 * QT;
   static constexpr uint32_t misc_off = bar_off + n_bars * 8;
   static constexpr uint32_t total = misc_off + 16;
 };
@@ -77,9 +77,9 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   auto bar_verdict = [&]() { return bars + 16u; };
   auto bar_packed_full = [&](int s) { return bars + 8u * (3 + s); };
   auto bar_packed_empty = [&](int s) { return bars + 8u * (3 + kPackedStages + s); };
-  auto bar_tile_full = [&](int s) { return bars + 8u * (3 + 2 * kPackedStages + s); };
-  auto bar_tile_empty = [&](int s) { return bars + 8u * (3 + 2 * kPackedStages + kTileStages + s); };
-  constexpr int kFirst = 3 + 2 * kPackedStages + 2 * kTileStages;
+  auto bar_tile_full = [&](int s, int v) { return bars + 8u * (3 + 2 * kPackedStages + 2 * s + v); };      // v: 0 K, 1 V
+  auto bar_tile_empty = [&](int s, int v) { return bars + 8u * (3 + 2 * kPackedStages + 2 * kTileStages + 2 * s + v); };
+  constexpr int kFirst = 3 + 2 * kPackedStages + 4 * kTileStages;
   auto bar_s_full = [&](int t) { return bars + 8u * (kFirst + 6 * t + 0); };
   auto bar_s_empty = [&](int t) { return bars + 8u * (kFirst + 6 * t + 1); };
   auto bar_p_full = [&](int t, int half) { return bars + 8u * (kFirst + 6 * t + 2 + half); };
@@ -122,8 +122,10 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       mbar_init(bar_packed_empty(s), 4);
     }
     for (int s = 0; s < kTileStages; ++s) {
-      mbar_init(bar_tile_full(s), 4);
-      mbar_init(bar_tile_empty(s), QT);
+      for (int v = 0; v < 2; ++v) {
+        mbar_init(bar_tile_full(s, v), 4);
+        mbar_init(bar_tile_empty(s, v), QT);
+      }
     }
     for (int t = 0; t < QT; ++t) {
       mbar_init(bar_s_full(t), 1);
@@ -150,52 +152,78 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   // the verdict: behind the first pass, or as soon as the running maximum is chosen from the start (a short range may be unpacked before that).
   auto again = [&]() -> bool { return mbar_wait(bar_verdict(), 0, cta_abort, a.status) && *cta_redo != 0; };
 
-  // Valid rows of block g; `rows`: rows that the block holds in memory.
-  auto block_rows = [&](int g, int& page_index, int& block, int& rows) -> int {
-    page_index = g / a.blocks_per_page;
-    block = g - page_index * a.blocks_per_page;
-    rows = block < a.full_blocks ? kFp4Rows : a.tail_rows;
-    return min((page_index == a.n_pages - 1 ? a.last_page_len : a.page_len) - block * kFp4Rows, kFp4Rows);
+  // Where a role is in its range: the page, the block in it and how many blocks of the page are left, this one included.
+  struct Place {
+    int page, block, left;
   };
+  auto blocks_of = [&](int page) { return page == a.n_pages - 1 ? a.total_blocks - page * a.blocks_per_page : a.blocks_per_page; };
+  auto first_place = [&]() -> Place {
+    const int page = g0 / a.blocks_per_page, block = g0 - page * a.blocks_per_page;
+    return {page, block, blocks_of(page) - block};
+  };
+  auto advance = [&](Place& p) {
+    ++p.block;
+    if (--p.left == 0) p = {p.page + 1, 0, blocks_of(p.page + 1)};
+  };
+  // rows that block `block` of a page holds in memory, and those of it that are valid
+  auto rows_of = [&](const Place& p) { return p.block < a.full_blocks ? kFp4Rows : a.tail_rows; };
+  auto valid_of = [&](const Place& p) { return p.left > 1 ? kFp4Rows : (p.page == a.n_pages - 1 ? a.last_page_len : a.page_len) - p.block * kFp4Rows; };
 
   if (warp >= kFirstUnpackWarp) {
     // =========================== dequantising warps ===========================
     if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4UnpackRegs));
-    const int tid = threadIdx.x - 32 * kFirstUnpackWarp;
-    for (int i = 0, end = 2 * nblk; i < end || (i == 2 * nblk && again() && (end = 4 * nblk)); ++i) {
-      int pi, block, rows;
-      const int valid = block_rows(g0 + (i >> 1) - (i >= 2 * nblk ? nblk : 0), pi, block, rows);
-      const int ps = i % kPackedStages, ts = i % kTileStages;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar_packed_full(ps), (i / kPackedStages) & 1, cta_abort, a.status) &&
-                                       mbar_wait(bar_tile_empty(ts), ((i / kTileStages) & 1) ^ 1u, cta_abort, a.status)))
-        break;
-      const uint8_t* from = smem + L::packed_off + ps * kPackedBytes;
-      const uint32_t to = sbase + L::tile_off + ts * kTileBytes;
-      // half rows in order: loads are 16 consecutive bytes a thread; eight threads store to four rows and both their halves, which the
-      // swizzle puts into eight different 16-byte columns
+    // A thread takes half rows (sixteen bytes, 32 values) of rows tid / 2 and 64 further on: loads are consecutive, and eight threads
+    // store to four rows and both their halves, which the swizzle puts into eight different 16-byte columns.
+    const int tid = threadIdx.x - 32 * kFirstUnpackWarp, row = tid >> 1;
+    const uint32_t to0 = sbase + L::tile_off + row * 128 + ((((tid & 1) * 4) ^ (row & 7)) << 4);
+    auto unpack = [&](const uint8_t* from, uint32_t to, int rows, int valid) {
+      uint4 w[2];
+      uint32_t scales[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = (tid + 128 * u) >> 1, half = tid & 1;
-        const uint4 w = *reinterpret_cast<const uint4*>(from + row * 32 + half * 16);
-        uint32_t both = *reinterpret_cast<const uint16_t*>(from + rows * 32 + row * 4 + half * 2);
-        if (row >= valid) both = 0;
-        const uint32_t s0 = (both & 0xffu) * 0x00800080u, s1 = (both >> 8) * 0x00800080u;
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        w[u] = *reinterpret_cast<const uint4*>(from + tid * 16 + u * 2048);
+        scales[u] = *reinterpret_cast<const uint16_t*>(from + rows * 32 + tid * 2 + u * 256);
+      }
+      if (valid < kFp4Rows) {
+        if (row >= valid) scales[0] = 0;
+        if (row + 64 >= valid) scales[1] = 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t s0 = (scales[u] & 0xffu) * 0x00800080u, s1 = (scales[u] >> 8) * 0x00800080u;
+        const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t p[4];
           fp4_unpack8(words[e], p);
           const uint32_t s = e < 2 ? s0 : s1;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + row * 128 + (((half * 4 + e) ^ (row & 7)) << 4)), "r"(half2_mul(p[0], s)),
-                       "r"(half2_mul(p[1], s)), "r"(half2_mul(p[2], s)), "r"(half2_mul(p[3], s))
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((to ^ (e << 4)) + u * 8192), "r"(half2_mul(p[0], s)), "r"(half2_mul(p[1], s)),
+                       "r"(half2_mul(p[2], s)), "r"(half2_mul(p[3], s))
                        : "memory");
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, a.status)); };
+    Place at = first_place();
+    for (int j = 0, end = nblk; j < end; ++j) {
+      const int ps = j % kPackedStages, ts = j % kTileStages, rows = rows_of(at), valid = valid_of(at);
+      const uint8_t* from = smem + L::packed_off + ps * 2 * kPackedBytes;
+      const uint32_t to = to0 + ts * 2 * kTileBytes, empty = ((j / kTileStages) & 1) ^ 1u;
+      if (!wait(bar_packed_full(ps), (j / kPackedStages) & 1) || !wait(bar_tile_empty(ts, 0), empty)) break;
+      unpack(from, to, rows, valid);
+      if (lane == 0) mbar_arrive(bar_tile_full(ts, 0));
+      if (!wait(bar_tile_empty(ts, 1), empty)) break;
+      unpack(from + kPackedBytes, to + kTileBytes, rows, valid);
       if (lane == 0) {
+        mbar_arrive(bar_tile_full(ts, 1));
         mbar_arrive(bar_packed_empty(ps));
-        mbar_arrive(bar_tile_full(ts));
+      }
+      advance(at);
+      if (j + 1 == nblk && __all_sync(0xffffffffu, again())) {
+        end = 2 * nblk;
+        at = first_place();
       }
     }
   } else if (warp == kProducerWarp) {
@@ -206,12 +234,11 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       for (int t = 0; t < QT; ++t) tma_load_4d(sbase + L::q_off + t * kTileBytes, &tm_q, bar_q_full(), 0, h, (qg * QT + t) * kTileM, 0);
       int cur = -1;
       const uint8_t* base = nullptr;
-      for (int i = 0, end = 2 * nblk; i < end || (i == 2 * nblk && again() && (end = 4 * nblk)); ++i) {
-        int pi, block, rows;
-        block_rows(g0 + (i >> 1) - (i >= 2 * nblk ? nblk : 0), pi, block, rows);
-        if (pi != cur) {
-          const int page = __ldg(a.page_table + pi);
-          cur = pi;
+      Place at = first_place();
+      for (int j = 0, end = nblk; j < end; ++j) {
+        if (at.page != cur) {
+          cur = at.page;
+          const int page = __ldg(a.page_table + cur);
           if (page < 0 || page >= a.num_pages) {
             atomicCAS(a.status, 0, kStatusBadIndex);
             *cta_abort = 1;
@@ -219,12 +246,18 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           }
           base = a.pool + (static_cast<int64_t>(page) * 2 * a.heads + h) * a.head_bytes;
         }
-        const int ps = i % kPackedStages;
-        if (!mbar_wait(bar_packed_empty(ps), ((i / kPackedStages) & 1) ^ 1u, cta_abort, a.status)) break;
-        const uint32_t bytes = rows * kFp4RowBytes<64>;
-        mbar_arrive_expect_tx(bar_packed_full(ps), bytes);
-        bulk_load(sbase + L::packed_off + ps * kPackedBytes, base + (i & 1) * a.heads * a.head_bytes + static_cast<int64_t>(block) * kPackedBytes, bytes,
-                  bar_packed_full(ps));
+        const int ps = j % kPackedStages;
+        if (!mbar_wait(bar_packed_empty(ps), ((j / kPackedStages) & 1) ^ 1u, cta_abort, a.status)) break;
+        const uint32_t bytes = rows_of(at) * kFp4RowBytes<64>, to = sbase + L::packed_off + ps * 2 * kPackedBytes;
+        const uint8_t* from = base + static_cast<int64_t>(at.block) * kPackedBytes;
+        mbar_arrive_expect_tx(bar_packed_full(ps), 2 * bytes);
+        bulk_load(to, from, bytes, bar_packed_full(ps));
+        bulk_load(to + kPackedBytes, from + a.heads * a.head_bytes, bytes, bar_packed_full(ps));
+        advance(at);
+        if (j + 1 == nblk && again()) {
+          end = 2 * nblk;
+          at = first_place();
+        }
       }
     }
   } else if (warp > kProducerWarp) {
@@ -233,17 +266,15 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     const int t = warp - kFirstMmaWarp;
     if (t < QT) {
       const uint32_t lead = elect_one();
-      auto k_stage = [](int j) { return (2 * j) % kTileStages; };
-      auto v_stage = [](int j) { return (2 * j + 1) % kTileStages; };
-      auto tile_parity = [](int j) -> uint32_t { return (2 * j / kTileStages) & 1; };
+      auto tile_parity = [](int j) -> uint32_t { return (j / kTileStages) & 1; };
       auto issue_s = [&](int s) {
         const uint64_t ad = smem_desc(sbase + L::q_off + t * kTileBytes, 16, 1024);
-        const uint64_t bd = smem_desc(sbase + L::tile_off + s * kTileBytes, 16, 1024);
+        const uint64_t bd = smem_desc(sbase + L::tile_off + s * 2 * kTileBytes, 16, 1024);
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_ss(lead, tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS16, k > 0);
       };
       auto issue_pv = [&](int s, int half, uint32_t accumulate) {
-        const uint64_t bd = smem_desc(sbase + L::tile_off + s * kTileBytes, 16, 1024);
+        const uint64_t bd = smem_desc(sbase + L::tile_off + (2 * s + 1) * kTileBytes, 16, 1024);
 #pragma unroll
         for (int k = 4 * half; k < 4 * half + 4; ++k)
           umma_ts(lead, tmem_base + kOCol + t * 64, tmem_base + kPCol + t * 64 + k * 8, bd + k * 128, kIdescPV16, k > 0 ? 1u : accumulate);
@@ -251,13 +282,13 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, a.status)); };
       // block j of all passes; S_j may overwrite S_{j-1} once that is in registers
       auto start_s = [&](int j) -> bool {
-        const int s = k_stage(j);
+        const int s = j % kTileStages;
         if (j > 0 && !wait(bar_s_empty(t), (j - 1) & 1)) return false;
-        if (!wait(bar_tile_full(s), tile_parity(j))) return false;
+        if (!wait(bar_tile_full(s, 0), tile_parity(j))) return false;
         tc_fence_after();
         issue_s(s);
         tc_commit_elected(lead, bar_s_full(t));
-        tc_commit_elected(lead, bar_tile_empty(s));
+        tc_commit_elected(lead, bar_tile_empty(s, 0));
         return true;
       };
       bool ok = wait(bar_q_ready(), 0);
@@ -266,10 +297,10 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
         ok = start_s(first);
         for (int j = first; ok && j < first + nblk; ++j) {
           if (j + 1 < first + nblk && !(ok = start_s(j + 1))) break;
-          const int s = v_stage(j);
+          const int s = j % kTileStages;
           if (!(ok = wait(bar_p_full(t, 0), j & 1))) break;
           if (both && !(ok = wait(bar_p_full(t, 1), j & 1))) break;
-          if (!(ok = wait(bar_tile_full(s), tile_parity(j)))) break;
+          if (!(ok = wait(bar_tile_full(s, 1), tile_parity(j)))) break;
           tc_fence_after();
           issue_pv(s, 0, j > first ? 1u : 0u);
           tc_commit_elected(lead, bar_pv_full(t, 0));
@@ -279,7 +310,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           }
           issue_pv(s, 1, 1u);
           tc_commit_elected(lead, bar_pv_full(t, 1));
-          tc_commit_elected(lead, bar_tile_empty(s));
+          tc_commit_elected(lead, bar_tile_empty(s, 1));
         }
         if (!ok || both || first > 0 || !__all_sync(0xffffffffu, again())) break;
         first = nblk;
@@ -363,7 +394,6 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     float m = -INFINITY, l = 0.f;                          // m: reference maximum (units of S); l: sum over this half
 
     int pi, left;
-    auto blocks_of = [&](int page) { return page == a.n_pages - 1 ? a.total_blocks - page * a.blocks_per_page : a.blocks_per_page; };
     auto rewind = [&]() {
       pi = g0 / a.blocks_per_page;
       left = blocks_of(pi) - (g0 - pi * a.blocks_per_page);
