@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           mask(s, valid);
           l += sweep(s, pk, shift, Yes(), integral_constant<int, 0>(), integral_constant<int, 1>());
         } else {
-          l += sweep(s, pk, shift, No(), integral_constant<int, 2>(), integral_constant<int, 5>());
+          l += sweep(s, pk, shift, No(), integral_constant<int, 1>(), integral_constant<int, 4>());
         }
         if (j > 0) {
           if (!(ok = wait_u(bar_pv_full(t, half), (j - 1) & 1))) break;
