@@ -12,6 +12,7 @@
 // clocks of issue.  Q is brought to half precision once per CTA: each row times the power of two that puts its largest value into
 // [2^14, 2^15) - bf16 queries lose nothing that an fp32 sum would keep - and the row's factor goes back into the multiply-add in front
 // of its exponential.  Weights are half-precision numbers of up to 2^15: eleven bits where bf16 has eight.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -66,7 +67,8 @@ struct Fp4Args {
 };
 
 template <int QT>
-__global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const __grid_constant__ CUtensorMap tm_q, const Fp4Args a) {
+__global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const __grid_constant__ CUtensorMap tm_q, const Fp4Args a,
+                                                                              const __grid_constant__ Fp4Pages pages) {
   using L = Fp4Smem<QT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       for (int j = 0, end = nblk; j < end; ++j) {
         if (at.page != cur) {
           cur = at.page;
-          const int page = __ldg(a.page_table + cur);
+          const int page = a.page_table == nullptr ? pages.id[cur] : __ldg(a.page_table + cur);
           if (page < 0 || page >= a.num_pages) {
             atomicCAS(a.status, 0, kStatusBadIndex);
             *cta_abort = 1;
@@ -631,9 +633,9 @@ int prepare_device() {
 
 }  // namespace
 
-int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, cudaStream_t stream) {
+int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, const int32_t* page_ids, cudaStream_t stream) {
   if (a.n_q <= 0 || a.heads <= 0 || a.batch != 1 || a.n_pages <= 0 || a.page_len <= 0 || a.last_page_len <= 0 || a.last_page_len > a.page_len ||
-      pool == nullptr || a.page_table == nullptr || a.status == nullptr || (a.q_tiles_per_cta != 1 && a.q_tiles_per_cta != 2))
+      pool == nullptr || (a.page_table == nullptr && page_ids == nullptr) || a.status == nullptr || (a.q_tiles_per_cta != 1 && a.q_tiles_per_cta != 2))
     return fail(GCT_ERR_INVALID, "attention: bad shape");
   Fp4Args k = {};
   k.pool = pool;
@@ -673,10 +675,16 @@ int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layo
   const int rc = prepare_device();
   if (rc != GCT_OK) return rc;
   const dim3 g(static_cast<unsigned>(grid));
+  Fp4Pages pages = {};
+  if (page_ids != nullptr) {
+    if (a.n_pages > kFp4ArgPages) return fail(GCT_ERR_INVALID, "attention: too many pages for an argument");
+    std::copy(page_ids, page_ids + a.n_pages, pages.id);
+    k.page_table = nullptr;
+  }
   if (a.q_tiles_per_cta == 2)
-    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<2>, g, dim3(kFp4Threads<2>), Fp4Smem<2>::total + 1024, stream, a.tm_q, k));
+    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<2>, g, dim3(kFp4Threads<2>), Fp4Smem<2>::total + 1024, stream, a.tm_q, k, pages));
   else
-    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<1>, g, dim3(kFp4Threads<1>), Fp4Smem<1>::total + 1024, stream, a.tm_q, k));
+    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<1>, g, dim3(kFp4Threads<1>), Fp4Smem<1>::total + 1024, stream, a.tm_q, k, pages));
   return GCT_OK;
 }
 

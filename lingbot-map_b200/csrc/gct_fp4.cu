@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "gct_fp4.h"
 #include "gct_sm100.h"
@@ -124,31 +125,46 @@ __global__ void __launch_bounds__(128) gct_fp4_rows_append_kernel(const float* _
 // cache and the call's own new rows.  There is almost nothing to compute: a call reads every row of the cache once (4.5 bits a value), so
 // what counts is how few instructions a value costs between its arrival and the sum.
 //
-//  * Four warps take 32 of a block's 128 keys each; a fifth fetches blocks (one bulk copy for K, one for V) into a ring of stages.
-//  * Products on mma.sync m16n8k16 in half precision, fp32 sums.  Queries are the sixteen rows: the upper eight hold q rounded to half
-//    precision, the lower eight what the rounding left, so the sum of both halves is a product with 22 bits of q (q is brought to
-//    [2^14, 2^15) by a power of two per row).  The same with the weights: exp2(x - max + 15) and its rest.  The sixteen rows cost no more
-//    than eight would: results agree with fp32 arithmetic to about 2^-21.
+//  * Four warps compute; a fifth fetches blocks (one bulk copy for K, one for V) into a ring of stages.
+//  * Products on mma.sync m16n8k16 in half precision, fp32 sums.  q k^T has the queries as its sixteen rows: the upper eight hold q rounded
+//    to half precision, the lower eight what the rounding left, so the sum of both halves is a product with 22 bits of q (q is brought to
+//    [2^14, 2^15) by a power of two per row) at the price of one.  (p v)^T has d as its rows and the queries as its eight columns, once with
+//    the weights exp2(x - max + 15) and once with their rests.  Results agree with fp32 arithmetic to about 2^-21.  With the queries as rows
+//    of p v its sums took twice the registers.  The paged cache's calls take bf16 queries, which leave no rest, and give bf16 results, for
+//    which a weight's eleven bits are enough (2^-12 of sum p |v|, a sixteenth of the result's own rounding): no rests there.
 //  * Any order of d is right for q k^T and any order of keys and of d for p v, as long as both operands agree.  A lane takes a
 //    quarter row of K as one 8- or 16-byte load (the d that it multiplies are its own), and of V an eighth of a row of the keys t, t+4,
-//    t+8, t+12: keys are numbered so that the sixteen logits of a lane's query are, without an exchange, the left operand of p v.
+//    t+8, t+12: keys are numbered so that the logits of a lane's query are, without an exchange, the right operand of (p v)^T.
 //  * V's operand pairs two keys at one d.  Two words of two keys are woven into words whose bytes hold (key a, key b) with two logical
 //    operations and a shift each, before a single conversion makes the pair; a weave after the conversion costs twice that.
 constexpr int kRowsWarps = 4;
+// Keys of a block that a warp takes per turn.  64: two pairs of warps take blocks by turns, which halves what a warp does once per turn (the
+// wait, maximum, vote and shift: some seventy instructions beside five a key); one query over 131,928 tokens 60.5 us with 32, 47.8 with 64.
+// 32: all four warps share a block; right for the camera head's short ranges of a few blocks per CTA (1,000 cached tokens 9.2 us, with 64 11.9).
+template <bool kPaged>
+constexpr int kTurnKeys = kPaged ? 64 : 32;
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr float kWeightShift = 15.f;       // weights are at most 2^15
 
+// CTAs that share an SM: five warps of 96 (128) registers each, and 41 (74) KB.  Five CTAs at D = 64 (72 registers, 32 bytes spilled): one query
+// over 131,928 tokens 50.6 us, with four 46.4.
 template <int D>
+constexpr int kRowsCtas = D == 64 ? 4 : 3;
+
+template <int D, bool kPaged>
 struct RowsSmem {
   static constexpr int kStages = D == 64 ? 4 : 3;
   static constexpr int kBlock = kFp4BlockBytes<D>;
   static constexpr int new_off = kStages * 2 * kBlock;            // the call's own rows, a block of K and one of V
-  static constexpr int stat_off = new_off + 2 * kBlock;           // [warps][8] maximum and sum
+  static constexpr int new_bytes = kPaged ? 0 : 2 * kBlock;
+  static constexpr int stat_off = new_off + new_bytes;            // [warps][8] maximum and sum
   static constexpr int bar_off = stat_off + kRowsWarps * 8 * 2 * 4;
   static constexpr int misc_off = bar_off + 2 * kStages * 8;
   static constexpr int total = misc_off + 16;
   static constexpr int out_off = 0;                               // [warps][8][D] partial outputs, over the ring when it has been read
   static_assert(kRowsWarps * 8 * D * 4 <= new_off, "partial outputs do not fit the ring");
+  // the merge of the key ranges: sums of at most 256 lanes over the ring
+  static_assert(8 * D / 4 * 32 <= new_off && 128 * 32 <= new_off, "lane sums do not fit the ring");
 };
 
 struct RowsArgs {
@@ -182,9 +198,10 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
 }
 
 template <int D, bool kPaged>
-__global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_kernel(const RowsArgs a) {
-  using L = RowsSmem<D>;
-  constexpr int kStages = L::kStages, kBlock = L::kBlock, kSteps = D / 16, kTiles = D / 8, kWords = D / 32;      // words: of a quarter row
+__global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kernel(const RowsArgs a, const __grid_constant__ Fp4Pages pages) {
+  using L = RowsSmem<D, kPaged>;
+  constexpr bool kRest = !kPaged;                // the second half-precision part of queries and weights
+  constexpr int kKeys = kTurnKeys<kPaged>, kStages = L::kStages, kBlock = L::kBlock, kSteps = D / 16, kTiles = D / 16, kWords = D / 32;      // words: of a quarter row
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t bars = smem_u32(smem + L::bar_off);
   auto bar_full = [&](int s) { return bars + 8u * s; };
@@ -203,50 +220,65 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_ke
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full(s), 1);
-      mbar_init(bar_empty(s), kRowsWarps);
+      mbar_init(bar_empty(s), kKeys / 32 == 2 ? 2 : kRowsWarps);
     }
     *cta_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  // Under the end of the kernel before, which leaves the memory idle: the first blocks of the range on their way to L2.  A hint that reads
+  // nothing, so it may be given for rows that kernel is still writing.
+  if constexpr (!kPaged) {
+    if (threadIdx.x < 2 * kStages && static_cast<int>(threadIdx.x >> 1) < g1 - g0) {
+      const uint8_t* from = (threadIdx.x & 1 ? a.cache_v : a.cache_k) + h * a.head_bytes + static_cast<int64_t>(g0 + (threadIdx.x >> 1)) * kBlock;
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(kBlock) : "memory");
+    }
+  }
   pdl_wait();
 
   if (warp == kRowsWarps) {
     // =========================== producer ===========================
     if (lane == 0) {
-      int page = 0, cur = -1;
-      for (int g = g0; g < g1; ++g) {
-        const int j = g - g0, s = j % kStages;
-        int block = g;
-        const uint8_t *k, *v;
+      int pi = 0, block = g0;
+      if constexpr (kPaged) {
+        pi = block / a.blocks_per_page;
+        block -= pi * a.blocks_per_page;
+      }
+      const uint8_t* k = a.cache_k + h * a.head_bytes;
+      const uint8_t* v = a.cache_v + h * a.head_bytes;
+      for (int j = 0; j < g1 - g0; ++j) {
+        const int s = j % kStages;
         if constexpr (kPaged) {
-          const int pi = g / a.blocks_per_page;
-          block = g - pi * a.blocks_per_page;
-          if (pi != cur) {
-            page = __ldg(a.page_table + pi);
-            cur = pi;
+          if (j == 0 || block == 0) {
+            const int page = a.page_table == nullptr ? pages.id[pi] : __ldg(a.page_table + pi);
             if (page < 0 || page >= a.num_pages) {
               atomicCAS(a.status, 0, kStatusBadIndex);
               *cta_abort = 1;
               break;
             }
+            k = a.pool + (static_cast<int64_t>(page) * 2 * a.heads + h) * a.head_bytes;
+            v = k + a.heads * a.head_bytes;
           }
-          k = a.pool + (static_cast<int64_t>(page) * 2 * a.heads + h) * a.head_bytes;
-          v = k + a.heads * a.head_bytes;
-        } else {
-          k = a.cache_k + h * a.head_bytes;
-          v = a.cache_v + h * a.head_bytes;
         }
-        if (!mbar_wait(bar_empty(s), ((j / kStages) & 1) ^ 1u, cta_abort, a.status)) break;
+        // naps between looks: spinning, the four fetching warps of an SM took one issue slot in eight
+        if (j >= kStages) {
+          for (int naps = 0; naps < 64 && !mbar_try_wait(bar_empty(s), ((j / kStages) & 1) ^ 1u); ++naps) __nanosleep(64);
+          if (!mbar_wait(bar_empty(s), ((j / kStages) & 1) ^ 1u, cta_abort, a.status)) break;
+        }
         const uint32_t bytes = (block < a.full_blocks ? kFp4Rows : a.tail_rows) * kFp4RowBytes<D>;
         const int64_t off = static_cast<int64_t>(block) * kBlock;
         mbar_arrive_expect_tx(bar_full(s), 2 * bytes);
         bulk_load(smem_u32(smem + s * 2 * kBlock), k + off, bytes, bar_full(s));
         bulk_load(smem_u32(smem + s * 2 * kBlock + kBlock), v + off, bytes, bar_full(s));
+        ++block;
+        if (kPaged && block == a.blocks_per_page) {
+          block = 0;
+          ++pi;
+        }
       }
     }
   } else {
-    // =========================== four warps of 32 keys each ===========================
+    // =========================== computing warps ===========================
     const int g = lane >> 2, t = lane & 3;
     const int row_q = group * 8 + g;
     // the quarter t of query row g, as the left operand: rows g (rounded) and g + 8 (the rest)
@@ -291,92 +323,124 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_ke
       c = a.scale_log2 / f;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        split_f16(x[4 * i] * f, x[4 * i + 1] * f, qf[i][0], qf[i][1]);
-        split_f16(x[4 * i + 2] * f, x[4 * i + 3] * f, qf[i][2], qf[i][3]);
+        if constexpr (kRest) {
+          split_f16(x[4 * i] * f, x[4 * i + 1] * f, qf[i][0], qf[i][1]);
+          split_f16(x[4 * i + 2] * f, x[4 * i + 3] * f, qf[i][2], qf[i][3]);
+        } else {                                           // bf16 queries are half-precision numbers as they are
+          qf[i][0] = pack_f16x2(x[4 * i] * f, x[4 * i + 1] * f);
+          qf[i][2] = pack_f16x2(x[4 * i + 2] * f, x[4 * i + 3] * f);
+          qf[i][1] = qf[i][3] = 0u;
+        }
       }
     }
+    // tile j of (p v)^T: d = (D / 8) g + 2 j and the one behind it, queries 2t and 2t + 1
     float acc[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     float m = -INFINITY, l = 0.f;          // of query row g: maximum of the base-2 exponents, sum of this lane's weights
 
-    // one block: `rows` rows of K at kb and of V at vb, the first `valid` of them count
-    auto use_block = [&](const uint8_t* kb, const uint8_t* vb, int rows, int valid) {
-      const int key0 = 32 * warp;
-      if (key0 >= valid) return;
-      float x[4][2];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
+    // kKeys keys from key0 on of a block with `rows` rows of K at kb and of V at vb, the first `valid` of which count
+    auto use_block = [&](const uint8_t* kb, const uint8_t* vb, int rows, int valid, int key0, auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;        // valid == 128
+      if (!kWhole && key0 >= valid) return;
+      float x[kKeys / 8][2];
+      {
         // column c of tile n is key 16 (n / 2) + 4 (c % 2 + 2 (n % 2)) + c / 2: those of a lane's weights are t, t + 4, t + 8, t + 12
-        const int key = key0 + 16 * (n >> 1) + 4 * ((g & 1) + 2 * (n & 1)) + (g >> 1);
-        uint32_t w[kWords], sc[kWords / 2];
+        const int key = key0 + 4 * (g & 1) + (g >> 1);
         const uint8_t* src = kb + key * (D / 2) + t * (D / 8);
         const uint8_t* ss = kb + rows * (D / 2) + key * (D / 16) + t * (D / 64);
-        if constexpr (D == 64) {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
-          w[0] = u.x; w[1] = u.y;
-          sc[0] = static_cast<uint32_t>(ss[0]) * 0x00800080u;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
-          w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-          const uint32_t both = *reinterpret_cast<const uint16_t*>(ss);
-          sc[0] = (both & 0xffu) * 0x00800080u;
-          sc[1] = (both >> 8) * 0x00800080u;
-        }
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          uint32_t b[4];
-          fp4_unpack8(w[i], b);
+        for (int n = 0; n < kKeys / 8; n += 2) {           // two tiles by turns: a product depends on the last but one
+          uint32_t w[2][kWords], sc[2][kWords / 2];
+          float d[2][4] = {};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = half2_mul(b[e], sc[i / 2]);
-          mma_f16(d, qf[2 * i], b[0], b[1]);
-          mma_f16(d, qf[2 * i + 1], b[2], b[3]);
+          for (int u = 0; u < 2; ++u) {
+            if constexpr (D == 64) {
+              const uint2 v = *reinterpret_cast<const uint2*>(src + 8 * (n + u) * (D / 2));
+              w[u][0] = v.x; w[u][1] = v.y;
+              sc[u][0] = static_cast<uint32_t>(ss[8 * (n + u) * (D / 16)]) * 0x00800080u;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(src + 8 * (n + u) * (D / 2));
+              w[u][0] = v.x; w[u][1] = v.y; w[u][2] = v.z; w[u][3] = v.w;
+              const uint32_t both = *reinterpret_cast<const uint16_t*>(ss + 8 * (n + u) * (D / 16));
+              sc[u][0] = (both & 0xffu) * 0x00800080u;
+              sc[u][1] = (both >> 8) * 0x00800080u;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            uint32_t b[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              fp4_unpack8(w[u][i], b[u]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) b[u][e] = half2_mul(b[u][e], sc[u][i / 2]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) mma_f16(d[u], qf[2 * i], b[u][0], b[u][1]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) mma_f16(d[u], qf[2 * i + 1], b[u][2], b[u][3]);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            x[n + u][0] = (kRest ? d[u][0] + d[u][2] : d[u][0]) * c;
+            x[n + u][1] = (kRest ? d[u][1] + d[u][3] : d[u][1]) * c;
+            if constexpr (!kWhole) {
+              const int mine = key0 + 8 * (n + u) + t;
+              if (mine >= valid) x[n + u][0] = -INFINITY;
+              if (mine + 4 >= valid) x[n + u][1] = -INFINITY;
+            }
+          }
         }
-        const int mine = key0 + 16 * (n >> 1) + 8 * (n & 1) + t;
-        x[n][0] = mine < valid ? (d[0] + d[2]) * c : -INFINITY;
-        x[n][1] = mine + 4 < valid ? (d[1] + d[3]) * c : -INFINITY;
       }
-      float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
+      float mx = fmaxf(x[0][0], x[0][1]);
+#pragma unroll
+      for (int n = 1; n < kKeys / 8; ++n) mx = max3(mx, x[n][0], x[n][1]);
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       if (__any_sync(0xffffffffu, mx > m)) {
         const float next = fmaxf(m, mx), alpha = next == -INFINITY ? 1.f : fast_exp2(m - next);
         m = next;
         l *= alpha;
+        const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);      // of queries 2t and 2t + 1
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] *= alpha;
+          acc[j][0] *= a0;
+          acc[j][1] *= a1;
+          acc[j][2] *= a0;
+          acc[j][3] *= a1;
         }
       }
       const float from = kWeightShift - (m == -INFINITY ? 0.f : m);
-      uint32_t p[2][4];
+      const int key = key0 + t;
+      const uint8_t* src = vb + key * (D / 2) + g * (D / 16);
+      const uint8_t* ss = vb + rows * (D / 2) + key * (D / 16) + (D == 64 ? g >> 1 : g);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float e0 = fast_exp2(x[n][0] + from), e1 = fast_exp2(x[n][1] + from);
-        l += e0 + e1;
-        split_f16(e0, e1, p[n >> 1][2 * (n & 1)], p[n >> 1][2 * (n & 1) + 1]);
-      }
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        const int key = key0 + 16 * step + t;
-        uint32_t w[4][kWords / 2], sc[4];
+      for (int step = 0; step < kKeys / 16; ++step) {
+        uint32_t w[4][kWords / 2], sc[4], p[2], rest[2];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int r = key + 4 * u;
-          const uint8_t* src = vb + r * (D / 2) + g * (D / 16);
-          const uint32_t s = vb[rows * (D / 2) + r * (D / 16) + (D == 64 ? g >> 1 : g)];
-          sc[u] = r < valid ? s << 7 : 0u;          // rows past the end count nothing, whatever they hold
+          const int r = 16 * step + 4 * u;
+          sc[u] = ss[r * (D / 16)];
+          if (!kWhole && key + r >= valid) sc[u] = 0;      // rows past the end count nothing, whatever they hold
           if constexpr (D == 64) {
-            w[u][0] = *reinterpret_cast<const uint32_t*>(src);
+            w[u][0] = *reinterpret_cast<const uint32_t*>(src + r * (D / 2));
           } else {
-            const uint2 both = *reinterpret_cast<const uint2*>(src);
+            const uint2 both = *reinterpret_cast<const uint2*>(src + r * (D / 2));
             w[u][0] = both.x;
             w[u][1] = both.y;
           }
         }
-        const uint32_t s01 = sc[0] | sc[1] << 16, s23 = sc[2] | sc[3] << 16;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float e0 = fast_exp2(x[2 * step + n][0] + from), e1 = fast_exp2(x[2 * step + n][1] + from);
+          l += e0 + e1;
+          if constexpr (kRest)
+            split_f16(e0, e1, p[n], rest[n]);
+          else
+            p[n] = pack_f16x2(e0, e1);
+        }
+        const uint32_t s01 = sc[0] << 7 | sc[1] << 23, s23 = sc[2] << 7 | sc[3] << 23;
 #pragma unroll
         for (int i = 0; i < kWords / 2; ++i) {
           constexpr uint32_t kLow = 0x0f0f0f0fu;
@@ -385,10 +449,18 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_ke
           fp4_unpack8(((w[0][i] >> 4) & kLow) | (w[1][i] & ~kLow), hi01);
           fp4_unpack8((w[2][i] & kLow) | ((w[3][i] << 4) & ~kLow), lo23);
           fp4_unpack8(((w[2][i] >> 4) & kLow) | (w[3][i] & ~kLow), hi23);
+          uint32_t v[4][4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            mma_f16(acc[8 * i + 2 * e], p[step], half2_mul(lo01[e], s01), half2_mul(lo23[e], s23));
-            mma_f16(acc[8 * i + 2 * e + 1], p[step], half2_mul(hi01[e], s01), half2_mul(hi23[e], s23));
+            v[e][0] = half2_mul(lo01[e], s01);
+            v[e][1] = half2_mul(hi01[e], s01);
+            v[e][2] = half2_mul(lo23[e], s23);
+            v[e][3] = half2_mul(hi23[e], s23);
+            mma_f16(acc[4 * i + e], v[e], p[0], p[1]);
+          }
+#pragma unroll
+          for (int e = 0; kRest && e < 4; ++e) {
+            mma_f16(acc[4 * i + e], v[e], rest[0], rest[1]);
           }
         }
       }
@@ -414,40 +486,54 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_ke
             }
           }
           asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory");
-          use_block(smem + L::new_off, smem + L::new_off + kBlock, kFp4Rows, rows);
+          // the last warp takes the first rows: the first has those of a short cache
+          use_block(smem + L::new_off, smem + L::new_off + kBlock, kFp4Rows, rows, 32 * (kRowsWarps - 1 - warp), std::false_type());
         }
       }
     }
-    for (int g = g0; g < g1; ++g) {
-      const int j = g - g0, s = j % kStages;
+    constexpr int kStep = kKeys == 64 ? 2 : 1;             // 64: a pair of warps takes every other block
+    const int pair = kKeys == 64 ? warp >> 1 : 0, key0 = kKeys == 64 ? 64 * (warp & 1) : 32 * warp;
+    int page = 0, block = g0 + pair;                       // place of the next block
+    if constexpr (kPaged) {
+      page = block / a.blocks_per_page;
+      block -= page * a.blocks_per_page;
+    }
+    for (int j = pair; j < g1 - g0; j += kStep) {
+      const int s = j % kStages;
       int rows = kFp4Rows, valid;
       if constexpr (kPaged) {
-        const int pi = g / a.blocks_per_page, block = g - pi * a.blocks_per_page;
         if (block >= a.full_blocks) rows = a.tail_rows;
-        valid = min((pi == a.n_pages - 1 ? a.last_page_rows : a.page_rows) - block * kFp4Rows, kFp4Rows);
+        valid = (page == a.n_pages - 1 ? a.last_page_rows : a.page_rows) - block * kFp4Rows;
+        block += kStep;
+        while (block >= a.blocks_per_page) {
+          block -= a.blocks_per_page;
+          ++page;
+        }
       } else {
-        valid = min(a.cached - g * kFp4Rows, kFp4Rows);
+        valid = a.cached - block * kFp4Rows;
+        block += kStep;
       }
       if (!__all_sync(0xffffffffu, mbar_wait(bar_full(s), (j / kStages) & 1, cta_abort, a.status))) break;
-      use_block(smem + s * 2 * kBlock, smem + s * 2 * kBlock + kBlock, rows, valid);
+      const uint8_t* at = smem + s * 2 * kBlock;
+      if (valid >= kFp4Rows)
+        use_block(at, at + kBlock, kFp4Rows, kFp4Rows, key0, std::true_type());
+      else
+        use_block(at, at + kBlock, rows, valid, key0, std::false_type());
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_empty(s));
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory");      // every warp has read its last stage
-    float* so = reinterpret_cast<float*>(smem + L::out_off) + (warp * 8 + g) * D;
-    // tile j holds d = (D / 8) n + j at column n; a lane's columns are 2t and 2t + 1
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      so[(D / 8) * (2 * t) + j] = acc[j][0] + acc[j][2];
-      so[(D / 8) * (2 * t + 1) + j] = acc[j][1] + acc[j][3];
+    for (int b = 0; b < 2; ++b) {
+      if (group * 8 + 2 * t + b < a.n_q) {
+        float* so = reinterpret_cast<float*>(smem + L::out_off) + (warp * 8 + 2 * t + b) * D + (D / 8) * g;
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 2) *reinterpret_cast<float4*>(so + 2 * j) = make_float4(acc[j][b], acc[j][2 + b], acc[j + 1][b], acc[j + 1][2 + b]);
+      }
     }
-    float* stat = reinterpret_cast<float*>(smem + L::stat_off) + (warp * 8 + g) * 2;
-    if (t == 0) {
-      stat[0] = m;
-      stat[1] = l;
-    }
+    if (t == 0) *reinterpret_cast<float2*>(smem + L::stat_off + (warp * 8 + g) * 8) = make_float2(m, l);
   }
   if (*cta_abort) {
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // copies in flight land before the shared memory is given up
@@ -502,27 +588,75 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 4 : 2) gct_fp4_rows_ke
   __syncthreads();
   if (!*is_last) return;
   __threadfence();
-  for (int e = threadIdx.x; e < rows_here * D; e += kRowsThreads) {
-    const int i = e / D, d = e % D;
-    const float* rec = a.part + (item * a.splits * 8 + i) * kRecord;
-    const size_t step = 8 * kRecord;
-    float mx = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, __ldcg(rec + s * step + D));
-    float num = 0.f, den = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-      const float ms = __ldcg(rec + s * step + D);
-      const float f = ms == mx ? 1.f : fast_exp2(ms - mx);
-      num = fmaf(f, __ldcg(rec + s * step + d), num);
-      den = fmaf(f, __ldcg(rec + s * step + D + 1), den);
+  // As many lanes per four columns as there are threads for (a power of two): each adds up every so many-th range against the largest
+  // maximum among them, then they are joined in order.  Maxima and sums come in one trip.
+  float4* lane_sum = reinterpret_cast<float4*>(smem);
+  const float* recs = a.part + item * a.splits * 8 * kRecord;
+  constexpr int kCols = D / 4, kAhead = 5;
+  const int items = rows_here * kCols;
+  int lanes = 1;
+  while (2 * lanes * items <= 128) lanes *= 2;
+  for (int e = threadIdx.x; e < items * lanes; e += kRowsThreads) {
+    const int it = e % items, ln = e / items, i = it / kCols, col = it % kCols;
+    float mx = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r0 = ln; r0 < a.splits; r0 += kAhead * lanes) {
+      float2 lo[kAhead], hi[kAhead], ml[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int r = r0 + u * lanes;
+        const float* rec = recs + (r * 8 + i) * kRecord;
+        ml[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + D)) : make_float2(-INFINITY, 0.f);
+        lo[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + 4 * col)) : make_float2(0.f, 0.f);
+        hi[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + 4 * col + 2)) : make_float2(0.f, 0.f);
+      }
+      float next = mx;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next = fmaxf(next, ml[u].x);
+      const float old = mx == next ? 1.f : fast_exp2(mx - next);
+      mx = next;
+      den *= old;
+      sum.x *= old;
+      sum.y *= old;
+      sum.z *= old;
+      sum.w *= old;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float f = ml[u].x == mx ? 1.f : fast_exp2(ml[u].x - mx);
+        den = fmaf(f, ml[u].y, den);
+        sum.x = fmaf(f, lo[u].x, sum.x);
+        sum.y = fmaf(f, lo[u].y, sum.y);
+        sum.z = fmaf(f, hi[u].x, sum.z);
+        sum.w = fmaf(f, hi[u].y, sum.w);
+      }
     }
-    finish(i, d, mx, num, den);
+    lane_sum[2 * e] = sum;
+    lane_sum[2 * e + 1] = make_float4(mx, den, 0.f, 0.f);
+  }
+  __syncthreads();
+  for (int it = threadIdx.x; it < items; it += kRowsThreads) {
+    float mx = -INFINITY, den = 0.f;
+    for (int ln = 0; ln < lanes; ++ln) mx = fmaxf(mx, lane_sum[2 * (it + ln * items) + 1].x);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int ln = 0; ln < lanes; ++ln) {
+      const float4 o = lane_sum[2 * (it + ln * items)], md = lane_sum[2 * (it + ln * items) + 1];
+      const float f = md.x == mx ? 1.f : fast_exp2(md.x - mx);
+      sum.x = fmaf(f, o.x, sum.x);
+      sum.y = fmaf(f, o.y, sum.y);
+      sum.z = fmaf(f, o.z, sum.z);
+      sum.w = fmaf(f, o.w, sum.w);
+      den = fmaf(f, md.y, den);
+    }
+    const int i = it / kCols, d = 4 * (it % kCols);
+    finish(i, d, mx, sum.x, den);
+    finish(i, d + 1, mx, sum.y, den);
+    finish(i, d + 2, mx, sum.z, den);
+    finish(i, d + 3, mx, sum.w, den);
   }
 }
 
 template <int D, bool kPaged>
-int launch_rows_kernel(const RowsArgs& k, dim3 grid, cudaStream_t stream) {
+int launch_rows_kernel(const RowsArgs& k, const Fp4Pages& pages, dim3 grid, cudaStream_t stream) {
   constexpr int kMaxDevices = 64;
   static std::mutex mu;
   static bool done[kMaxDevices] = {false};
@@ -532,11 +666,11 @@ int launch_rows_kernel(const RowsArgs& k, dim3 grid, cudaStream_t stream) {
   {
     std::lock_guard<std::mutex> lock(mu);
     if (!done[dev]) {
-      GCT_CUDA_CHECK(cudaFuncSetAttribute(gct_fp4_rows_kernel<D, kPaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D>::total));
+      GCT_CUDA_CHECK(cudaFuncSetAttribute(gct_fp4_rows_kernel<D, kPaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D, kPaged>::total));
       done[dev] = true;
     }
   }
-  GCT_CUDA_CHECK(launch_pdl(gct_fp4_rows_kernel<D, kPaged>, grid, dim3(kRowsThreads), RowsSmem<D>::total, stream, k));
+  GCT_CUDA_CHECK(launch_pdl(gct_fp4_rows_kernel<D, kPaged>, grid, dim3(kRowsThreads), RowsSmem<D, kPaged>::total, stream, k, pages));
   return GCT_OK;
 }
 
@@ -547,7 +681,7 @@ bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters) {
   const int64_t items = static_cast<int64_t>(groups) * heads;
   if (blocks <= 1 || items > num_counters) return 1;
-  const int64_t slots = static_cast<int64_t>(sms) * (head_dim == 64 ? 4 : 2);
+  const int64_t slots = static_cast<int64_t>(sms) * (head_dim == 64 ? kRowsCtas<64> : kRowsCtas<128>);
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / items, blocks));
   splits = std::min<int64_t>(splits, static_cast<int64_t>(part_floats / (static_cast<size_t>(items) * 8 * (head_dim + 2))));
   return static_cast<int>(std::max<int64_t>(splits, 1));
@@ -557,7 +691,7 @@ int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream) {
   if (p.q == nullptr || p.n_q <= 0 || p.heads <= 0 || p.status == nullptr || (p.head_dim != 64 && p.head_dim != 128))
     return fail(GCT_ERR_INVALID, "fp4 attention: bad argument");
   const bool paged = p.pool != nullptr;
-  if (paged ? p.page_table == nullptr || p.head_dim != 64 || p.n_pages <= 0 || p.page_rows <= 0 || p.last_page_rows <= 0 || p.last_page_rows > p.page_rows ||
+  if (paged ? (p.page_table == nullptr && p.page_ids == nullptr) || p.head_dim != 64 || p.n_pages <= 0 || p.page_rows <= 0 || p.last_page_rows <= 0 || p.last_page_rows > p.page_rows ||
                   p.n_new != 0
             : p.cache_k == nullptr || p.cache_v == nullptr || p.cached < 0 || p.n_new < 0 || p.cached + p.n_new <= 0 || p.layout.tail_rows != 0)
     return fail(GCT_ERR_INVALID, "fp4 attention: bad cache");
@@ -610,8 +744,14 @@ int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream) {
   const int64_t ctas = static_cast<int64_t>(k.groups) * k.splits * p.heads;
   if (ctas > 0x7fffffff) return fail(GCT_ERR_INVALID, "fp4 attention: too many rows");
   const dim3 grid(static_cast<unsigned>(ctas));
-  if (paged) return launch_rows_kernel<64, true>(k, grid, stream);
-  return p.head_dim == 64 ? launch_rows_kernel<64, false>(k, grid, stream) : launch_rows_kernel<128, false>(k, grid, stream);
+  Fp4Pages pages = {};
+  if (paged && p.page_ids != nullptr) {
+    if (p.n_pages > kFp4ArgPages) return fail(GCT_ERR_INVALID, "fp4 attention: too many pages for an argument");
+    std::copy(p.page_ids, p.page_ids + p.n_pages, pages.id);
+    k.page_table = nullptr;
+  }
+  if (paged) return launch_rows_kernel<64, true>(k, pages, grid, stream);
+  return p.head_dim == 64 ? launch_rows_kernel<64, false>(k, pages, grid, stream) : launch_rows_kernel<128, false>(k, pages, grid, stream);
 }
 
 int launch_fp4_read(const Fp4ReadLaunch& p, cudaStream_t stream) {
@@ -653,7 +793,7 @@ constexpr size_t kDecodeStatusBytes = 256;
 constexpr int kDecodeCounters = 2048;
 // Counters and partial results of one wave of CTAs; calls with more (head, eight queries) items than counters take one key range.
 size_t decode_fp4_workspace(int head_dim) {
-  return kDecodeStatusBytes + kDecodeCounters * sizeof(int) + static_cast<size_t>(148 * (head_dim == 64 ? 4 : 2)) * 8 * (head_dim + 2) * sizeof(float);
+  return kDecodeStatusBytes + kDecodeCounters * sizeof(int) + static_cast<size_t>(148 * (head_dim == 64 ? gct::kRowsCtas<64> : gct::kRowsCtas<128>)) * 8 * (head_dim + 2) * sizeof(float);
 }
 
 int check_decode_cache(const char* who, int heads, int head_dim, int capacity) {

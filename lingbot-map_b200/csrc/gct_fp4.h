@@ -123,6 +123,13 @@ int launch_scan_keys_fp4(const uint8_t* pool, int num_pages, int page_size, int 
 int launch_fp4_rows_append(const float* k, const float* v, int rows, uint8_t* cache_k, uint8_t* cache_v, const Fp4Layout& layout, int first,
                            int heads, int head_dim, cudaStream_t stream);
 
+// The pages of a plan as a kernel argument: it spares the copy of a table to the device ahead of each frame's first call (4 us of the
+// stream's time).  Longer plans use the table.
+constexpr int kFp4ArgPages = 256;
+struct Fp4Pages {
+  int32_t id[kFp4ArgPages];
+};
+
 // Attention of a few query rows (any number: eight at a time) over a 4-bit cache.
 struct Fp4RowsLaunch {
   const void* q = nullptr;               // [n_q, heads, D]
@@ -132,6 +139,7 @@ struct Fp4RowsLaunch {
   // paged: pool [pages][2][heads][layout.bytes], page_table; else cache_k / cache_v [heads][layout.bytes] with `cached` rows
   const uint8_t* pool = nullptr;
   const int32_t* page_table = nullptr;
+  const int32_t* page_ids = nullptr;     // the same on the host (at most kFp4ArgPages), used instead when given
   int n_pages = 0, num_pages = 0, page_rows = 0, last_page_rows = 0;
   uint8_t* cache_k = nullptr;
   uint8_t* cache_v = nullptr;
@@ -152,7 +160,8 @@ struct Fp4RowsLaunch {
 };
 int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream);
 // Attention of query tiles over a 4-bit pool; `a` as for launch_attention (tm_k, tm_v, key_norm_max and ctas_per_sm are not used).
-int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, cudaStream_t stream);
+// page_ids: as for Fp4RowsLaunch.
+int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, const int32_t* page_ids, cudaStream_t stream);
 // Key ranges that a call of `groups` x `heads` (head, eight queries) items over `blocks` blocks of 128 rows is cut into.
 int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters);
 

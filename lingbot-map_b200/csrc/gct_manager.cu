@@ -113,6 +113,7 @@ struct gct_mgr {
   // asynchronous copy (a pageable source would be staged by the runtime at call time)
   bool planned = false;
   int plan_pages = 0, plan_last_len = 0;
+  std::vector<int32_t> plan_ids;     // 4-bit cache, a plan of at most kFp4ArgPages pages: handed to the kernels as an argument (else empty)
   static constexpr int kPlanSlots = 8;
   int32_t* plan_ring = nullptr;                  // [kPlanSlots][max_num_pages], cudaHostAlloc
   cudaEvent_t plan_done[kPlanSlots] = {};        // recorded after the copy out of each slot
@@ -743,6 +744,14 @@ int gct_mgr_plan(gct_mgr_t* m, int page_begin, int page_end, void* stream) {
   const int last = (page_end == n) ? last_page_len(m, b) : m->geo.page_size;
   if (last < 1 || last > m->geo.page_size)                                                          // :394-396
     return fail(GCT_ERR_INVALID, "block 0: last_page_len=" + std::to_string(last) + " out of range");
+  m->plan_pages = page_end - page_begin;
+  m->plan_last_len = last;
+  m->plan_ids.clear();
+  if (m->fp4 && m->plan_pages <= kFp4ArgPages) {
+    m->plan_ids.assign(vis.begin() + page_begin, vis.begin() + page_end);
+    m->planned = true;
+    return GCT_OK;
+  }
   // pinned staging slot: reused every kPlanSlots plans, after the copy out of it has completed
   const int slot = static_cast<int>(m->plan_count++ % gct_mgr::kPlanSlots);
   if (m->plan_used[slot]) GCT_CUDA_CHECK(cudaEventSynchronize(m->plan_done[slot]));
@@ -752,8 +761,6 @@ int gct_mgr_plan(gct_mgr_t* m, int page_begin, int page_end, void* stream) {
                                  cudaMemcpyHostToDevice, static_cast<cudaStream_t>(stream)));
   GCT_CUDA_CHECK(cudaEventRecord(m->plan_done[slot], static_cast<cudaStream_t>(stream)));
   m->plan_used[slot] = true;
-  m->plan_pages = page_end - page_begin;
-  m->plan_last_len = last;
   m->planned = true;
   return GCT_OK;
 }
@@ -774,7 +781,8 @@ static int timed(gct_mgr* m, cudaStream_t stream, F&& launch) {
 }
 static int timed_attention(gct_mgr* m, int block, const AttnLaunch& a, cudaStream_t stream) {
   return timed(m, stream, [&] {
-    return m->fp4 ? launch_attention_fp4(a, m->pools4[block], m->fp4_page, m->geo.max_num_pages, stream) : launch_attention(a, stream);
+    return m->fp4 ? launch_attention_fp4(a, m->pools4[block], m->fp4_page, m->geo.max_num_pages, m->plan_ids.empty() ? nullptr : m->plan_ids.data(), stream)
+                  : launch_attention(a, stream);
   });
 }
 
@@ -796,6 +804,7 @@ static int run_paged_fp4(gct_mgr* m, int block, const void* q_dev, int q_dtype, 
   p.heads = m->cfg.num_heads;
   p.pool = m->pools4[block];
   p.page_table = m->table_dev;
+  p.page_ids = m->plan_ids.empty() ? nullptr : m->plan_ids.data();
   p.n_pages = m->plan_pages;
   p.num_pages = m->geo.max_num_pages;
   p.page_rows = m->geo.page_size;

@@ -247,6 +247,26 @@ def test_partial_results_of_page_ranges_merge():
         assert (np.abs(out - want) <= bound_frame(len(k), spread_of(q, k), weighted, want)).all()
 
 
+def test_plans_of_many_pages():
+    """More pages than a plan hands over as an argument: 500 frames on pages of seven rows; then few again after a reset."""
+    rs = np.random.RandomState(13)
+    m, k, v = filled(13, 2, 500, rs, scale=2, window=3)
+    assert len(m.build_visible_page_table(0)) > 256
+    for n_q in (1, 13):
+        q = bf(rs.standard_normal((n_q, 2, 64)))
+        want, _, weighted = F.attention(q, k, v)
+        for _ in range(2):
+            out = host(m.compute_attention(0, dev(q, torch.bfloat16)))
+            assert (np.abs(out - want) <= bound_frame(len(k), spread_of(q, k), weighted, want)).all()
+    m.reset()
+    x = dev(rs.standard_normal((13, 2, 64)), torch.bfloat16)
+    m.append_frame(0, x, x)
+    k, v = (host(t) for t in m._gather_kv(0))
+    want, _, weighted = F.attention(host(x), k, v)
+    assert (np.abs(host(m.compute_attention(0, x)) - want) <= bound_frame(len(k), spread_of(host(x), k), weighted, want)).all()
+    assert m.device_status() == 0
+
+
 def bound_frame(keys, spread, weighted, out):
     """Any path: as bound_rows, with weights rounded to half precision (2^-11 relative; below 2^-14 of their scale 2^-25 absolutely) and
     exponentials good to 2^-13 in numerator and denominator, and the merge of ranges in fp32."""
