@@ -185,7 +185,8 @@ __device__ __forceinline__ uint32_t fp4_block16(const float (&x)[16], int part, 
   }
   const uint32_t byte0 = fp4_scale_byte(max(top0, __shfl_xor_sync(0xffffffffu, top0, 1)));
   const uint32_t byte1 = fp4_scale_byte(max(top1, __shfl_xor_sync(0xffffffffu, top1, 1)));
-  const uint32_t w0 = fp4_pack8(b, fp4_scale(byte0)), w1 = fp4_pack8(b + 8, fp4_scale(byte1));
+  const float s0 = fp4_scale(byte0), s1 = fp4_scale(byte1);
+  const uint32_t w0 = fp4_pack8(b, s0, fp4_reciprocal(s0)), w1 = fp4_pack8(b + 8, s1, fp4_reciprocal(s1));
   const bool odd = part & 1;
   const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
   w[0] = odd ? other : w0;

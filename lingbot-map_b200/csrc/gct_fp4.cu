@@ -91,9 +91,9 @@ struct Fp4Group16 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = max(top, fp4_abs_bits(x[i]));
     scale = fp4_scale_byte(top);
-    const float s = fp4_scale(scale);
-    w[0] = fp4_pack8(x, s);
-    w[1] = fp4_pack8(x + 8, s);
+    const float s = fp4_scale(scale), r = fp4_reciprocal(s);
+    w[0] = fp4_pack8(x, s, r);
+    w[1] = fp4_pack8(x + 8, s, r);
   }
   __device__ __forceinline__ void store(uint8_t* values, uint8_t* scale_at) const {
     *reinterpret_cast<uint2*>(values) = make_uint2(w[0], w[1]);

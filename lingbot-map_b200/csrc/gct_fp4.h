@@ -66,18 +66,26 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t largest) {
   return ((u + 0x7ffffu + ((u >> 20) & 1u)) >> 20) - 8u * (127u - 15u);
 }
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7))); }
-__device__ __forceinline__ float fp4_quotient(float x, float s) { return s > 0.f ? __fdiv_rn(x, s) : 0.f; }
+// x / s rounded to the nearest, given r = 1 / s rounded to the nearest: a product and one correction by its residual (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990: with a correctly rounded reciprocal the corrected
+// quotient is correctly rounded, as long as the residual does not underflow; where it does here, x is far below s / 4 and becomes 0).  s = 0 or
+// NaN has r = 0, and every quotient is 0.
+__device__ __forceinline__ float fp4_reciprocal(float s) { return s > 0.f ? __frcp_rn(s) : 0.f; }
+__device__ __forceinline__ float fp4_quotient(float x, float s, float r) {
+  const float q = x * r;
+  return r > 0.f ? fmaf(fmaf(-q, s, x), r, q) : 0.f;
+}
 // Two quotients as two values of a byte, `lo` in its lower four bits.
 __device__ __forceinline__ uint32_t fp4_pack2(float lo, float hi) {
   uint32_t r;
   asm("{\n\t.reg .b8 b;\n\t.reg .b16 h;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tmov.b16 h, {b, 0};\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Eight values x with scale s (a NaN or zero scale: zeros).
-__device__ __forceinline__ uint32_t fp4_pack8(const float* x, float s) {
+// Eight values x with scale s and its reciprocal r (a NaN or zero scale: zeros).
+__device__ __forceinline__ uint32_t fp4_pack8(const float* x, float s, float r) {
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= fp4_pack2(fp4_quotient(x[2 * i], s), fp4_quotient(x[2 * i + 1], s)) << (8 * i);
+  for (int i = 0; i < 4; ++i) w |= fp4_pack2(fp4_quotient(x[2 * i], s, r), fp4_quotient(x[2 * i + 1], s, r)) << (8 * i);
   return w;
 }
 // The eight values of a word as four pairs of half-precision numbers, in order.

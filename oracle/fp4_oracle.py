@@ -29,7 +29,7 @@ def quantise(x):
     s = SCALES[byte]
     y = np.where((s > 0) & finite, 1.0, 0.0)[..., None] * np.abs(np.where(np.isfinite(b), b, 0.0)) / np.where(s > 0, s, 1.0)[..., None]
     code = _nearest(np.minimum(y, 6.0), VALUES)
-    negative = np.signbit(b) & ((s > 0) & finite)[..., None]
+    negative = (b < 0) & ((s > 0) & finite)[..., None]      # a negative zero is a zero
     return (code + 8 * negative).reshape(x.shape).astype(np.uint8), np.where(finite, byte, 255).astype(np.uint8)
 
 

@@ -103,6 +103,33 @@ def test_append_stores_the_quantised_rows(patches, H, ns, kd, vd):
     assert m.device_status() == 0
 
 
+def test_every_border_of_every_scale():
+    """Blocks of every scale with values on all seven borders between two codes, and on the fp32 numbers on either side of them."""
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    scales = F.SCALES[1:F.TOP_BYTE + 1]
+    blocks = []
+    for s in scales:
+        for step in (None, 0.0, np.inf):
+            x = (borders * s).astype(np.float32)
+            if step is not None:
+                x = np.nextafter(x, np.float32(step))
+            blocks.append(np.concatenate([[6 * s], x, -x, [0.0]]))
+    x = np.array(blocks)
+    x = np.concatenate([x, np.zeros((-len(x) % 8, 16))]).reshape(-1, 1, 128)
+    assert (F.SCALES[F.quantise(x)[1]].reshape(-1)[:3 * len(scales)].reshape(-1, 3) == scales[:, None]).all()
+    c = P.DecodeCache(1, 128, DEV, kv_bits=4)
+    c.append(dev(x), dev(-x))
+    got = c.rows_fp4(0, len(x))
+    same_rows(got[:2], x, "K")
+    same_rows(got[2:], -x, "V")
+    y = x.reshape(-1, 1, 64)                              # the paged cache: the same, rounded to bf16 first
+    m = manager(len(y), 1, ns=0)
+    m.append_frame(0, dev(y), dev(-y))
+    got = m.last_frame_fp4(0)
+    same_rows(got[:2], bf(y), "paged K")
+    same_rows(got[2:], bf(-y), "paged V")
+
+
 @pytest.mark.parametrize("src", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("mode,norm", [(_lib.ROPE_3D, True), (_lib.ROPE_2D, True), (_lib.ROPE_NONE, False), (_lib.ROPE_3D, False)])
 def test_fused_append_is_the_wide_append_quantised(src, mode, norm):
