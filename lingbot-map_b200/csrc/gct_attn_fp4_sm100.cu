@@ -2,16 +2,20 @@
 // accumulation.  The sibling of gct_attn_kernel (gct_attn_sm100.cu): the same tiles of 128 query rows, the same softmax with two threads per
 // row, the same split of the KV range over CTAs.  What differs is how K and V reach the tensor core.
 //
-//   producer warp      fetches blocks of 128 rows of K and V by turns, packed, one bulk copy each (4.6 KB), into a ring
-//   dequantising warps (four) turn a packed block into a 128 x 64 half-precision tile in the 128B-swizzled layout the products want: a
-//                      thread takes 32 values at a time, a conversion and a product with the scale per pair.  c * s is exact, rows past the
-//                      valid ones get scale zero, so nothing that they hold counts.
+//   producer warp      fetches blocks of 128 rows, packed (K and V, two bulk copies, 9.2 KB), into a ring
+//   unpacking warps    (four for K, four for V) turn a packed block into 128 x 64 half-precision tiles in the 128B-swizzled layout the
+//                      products want: a thread takes 32 values at a time, a conversion and a product with the scale per pair.  c * s is
+//                      exact; rows past the valid ones get scale zero, so nothing that they hold counts.
 //   MMA warps          S = Q K^T and O += P V, as there
+//   softmax warps      as there, 32 columns of S at a time, so that 88 registers do (64 at a time spilled: 10 % slower)
 //
-// A value costs its unpacking once per CTA, for the 256 query rows of two tiles: 16,384 values a block, about 170 of the block's 2,000
-// clocks of issue.  Q is brought to half precision once per CTA: each row times the power of two that puts its largest value into
-// [2^14, 2^15) - bf16 queries lose nothing that an fp32 sum would keep - and the row's factor goes back into the multiply-add in front
-// of its exponential.  Weights are half-precision numbers of up to 2^15: eleven bits where bf16 has eight.
+// A value costs its unpacking once per CTA, for the 256 query rows of two tiles: 16,384 values a block, about 800 of the block's 6,100 warp
+// instructions.  1005 queries over 131,928 tokens, kernel and merge back to back: 650 us (840 TFLOP/s; the bf16 cache 559); with four unpacking
+// warps 692, without the fifth K16 step (below) 688, unpacking by the softmax warps between their blocks 742, without any unpacking (wrong
+// results) 647 when the whole took 692.  What bounds it: as in gct_attn_kernel issue slots (packed f32x2 operations take two each) and the
+// chain S -> registers -> P -> P V; issue 64 % busy, tensor pipe 48 %.
+//
+// Weights are half-precision numbers of up to 2^15: eleven bits where bf16 has eight.  Q is brought to half precision once per CTA.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -26,16 +30,17 @@ constexpr int kPackedStages = 4, kTileStages = 2;          // blocks (K and V) i
 constexpr uint32_t kPackedBytes = kFp4BlockBytes<64>;
 constexpr float kFp4Shift = 7.f;                           // running maximum: weights are at most 2^(kRescaleThreshold + kFp4Shift)
 constexpr float kFixedShift = 15.f;                        // fixed reference: weights are at most 2^15
+constexpr int kFixedNum = 1, kFixedDen = 4;                // there, pairs of logits whose exponentials take the FMA pipe
 // half-precision operands: formats 0; K-major A and B for S, MN-major B for P V
 constexpr uint32_t kIdescS16 = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescPV16 = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
 
-// Warpgroups: two softmax per query tile, one of producer and MMA warps, one dequantising.
+// Warpgroups: two softmax per query tile, one of producer and MMA warps, two that unpack.
 template <int QT>
-constexpr int kFp4Threads = 256 * QT + 256;
-// Two tiles: 768 threads start with 80 registers each; 512 * 96 + 128 * 40 + 128 * 56 = 61440 = 768 * 80.
-constexpr int kFp4SoftmaxRegs = 96, kFp4ControlRegs = 40, kFp4UnpackRegs = 56;
-static_assert(512 * kFp4SoftmaxRegs + 128 * kFp4ControlRegs + 128 * kFp4UnpackRegs <= 768 * 80, "register pool of the CTA exceeded");
+constexpr int kFp4Threads = 256 * QT + 384;
+// Two tiles: 896 threads start with 72 registers each, 64512 in all.
+constexpr int kFp4SoftmaxRegs = 88, kFp4ControlRegs = 40, kFp4UnpackRegs = 56;
+static_assert(512 * kFp4SoftmaxRegs + 128 * kFp4ControlRegs + 256 * kFp4UnpackRegs <= 896 * 72, "register pool of the CTA exceeded");
 
 template <int QT>
 struct Fp4Smem {
@@ -45,11 +50,16 @@ struct Fp4Smem {
   static constexpr uint32_t pair_off = packed_off + kPackedStages * 2 * kPackedBytes;      // [2][QT][2][128] floats, as in gct_attn_kernel
   static constexpr uint32_t factor_off = pair_off + 2 * QT * 2 * 128 * 4;              // [QT][128] floats: a row's multiplier in front of exp2
   static constexpr uint32_t ref_off = factor_off + QT * 128 * 4;                       // [QT][128] floats: a row's fixed reference
-  static constexpr uint32_t bar_off = ref_off + QT * 128 * 4;
+  // operands of the fifth K16 step of S: columns [16 t, +16) Qx of tile t (column 0 = 15 - reference), [32, 48) Kx (column 0 = 1)
+  static constexpr uint32_t x_off = (ref_off + QT * 128 * 4 + 1023) / 1024 * 1024;
+  static constexpr uint32_t bar_off = x_off + kTileBytes;
   // q_full, q_ready, verdict, packed_full/empty[], K and V tile_full/empty[], per query tile s_full, s_empty, p_full[2], pv_full[2]
   static constexpr int n_bars = 3 + 2 * kPackedStages + 4 * kTileStages + 6 * QT;
   static constexpr uint32_t misc_off = bar_off + n_bars * 8;
-  static constexpr uint32_t total = misc_off + 16;
+  // [2 kTileStages] valid rows of an unpacked block.  K of block j is freed when S_j is done, which may be before the softmax has looked here;
+  // K of block j + 2 kTileStages is unpacked after S_{j + kTileStages}, which began after the softmax had left block j.
+  static constexpr uint32_t valid_off = misc_off + 16;
+  static constexpr uint32_t total = valid_off + 2 * kTileStages * 4;
 };
 
 struct Fp4Args {
@@ -66,7 +76,9 @@ struct Fp4Args {
   float fixed_limit;              // largest bound of a row's exponents that the fixed reference is tried with
 };
 
-template <int QT>
+// kFold: S arrives as the finished base-2 exponent, less the row's reference (bf16 results: the logits' rounding, 2^-12 relative to |q| |k| of
+// each product, is far below theirs); otherwise scale and reference enter by a multiply-add in fp32, for callers who want the log-sum-exp.
+template <int QT, bool kFold>
 __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const __grid_constant__ CUtensorMap tm_q, const Fp4Args a,
                                                                               const __grid_constant__ Fp4Pages pages) {
   using L = Fp4Smem<QT>;
@@ -121,7 +133,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     mbar_init(bar_verdict(), 8 * QT);
     for (int s = 0; s < kPackedStages; ++s) {
       mbar_init(bar_packed_full(s), 1);
-      mbar_init(bar_packed_empty(s), 4);
+      mbar_init(bar_packed_empty(s), 8);
     }
     for (int s = 0; s < kTileStages; ++s) {
       for (int v = 0; v < 2; ++v) {
@@ -154,31 +166,54 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
   // the verdict: behind the first pass, or as soon as the running maximum is chosen from the start (a short range may be unpacked before that).
   auto again = [&]() -> bool { return mbar_wait(bar_verdict(), 0, cta_abort, a.status) && *cta_redo != 0; };
 
-  // Where a role is in its range: the page, the block in it and how many blocks of the page are left, this one included.
+  // Where a role is in its range: the page, how many of its blocks are left, this one included, the rows that this block holds in memory and
+  // those of them that are valid.
   struct Place {
-    int page, block, left;
+    int page, left, rows, valid;
   };
   auto blocks_of = [&](int page) { return page == a.n_pages - 1 ? a.total_blocks - page * a.blocks_per_page : a.blocks_per_page; };
+  auto end_of_page = [&](Place& p) {                       // at the last block of a page
+    const int block = blocks_of(p.page) - 1;
+    p.rows = block < a.full_blocks ? kFp4Rows : a.tail_rows;
+    p.valid = (p.page == a.n_pages - 1 ? a.last_page_len : a.page_len) - block * kFp4Rows;
+  };
   auto first_place = [&]() -> Place {
-    const int page = g0 / a.blocks_per_page, block = g0 - page * a.blocks_per_page;
-    return {page, block, blocks_of(page) - block};
+    Place p = {g0 / a.blocks_per_page, 0, kFp4Rows, kFp4Rows};
+    p.left = blocks_of(p.page) - (g0 - p.page * a.blocks_per_page);
+    if (p.left == 1) end_of_page(p);
+    return p;
   };
   auto advance = [&](Place& p) {
-    ++p.block;
-    if (--p.left == 0) p = {p.page + 1, 0, blocks_of(p.page + 1)};
+    if (--p.left > 1) return;
+    if (p.left == 0) {
+      p = {p.page + 1, blocks_of(p.page + 1), kFp4Rows, kFp4Rows};
+      if (p.left > 1) return;
+    }
+    end_of_page(p);
   };
-  // rows that block `block` of a page holds in memory, and those of it that are valid
-  auto rows_of = [&](const Place& p) { return p.block < a.full_blocks ? kFp4Rows : a.tail_rows; };
-  auto valid_of = [&](const Place& p) { return p.left > 1 ? kFp4Rows : (p.page == a.n_pages - 1 ? a.last_page_len : a.page_len) - p.block * kFp4Rows; };
+  // keys of the range: whole blocks, less what the last block of each page that ends in it lacks
+  auto keys_of_range = [&]() -> int {
+    const int first = g0 / a.blocks_per_page, last = (g1 - 1) / a.blocks_per_page;
+    const bool whole = g1 == a.total_blocks || g1 % a.blocks_per_page == 0;      // the range's last page ends in it
+    const int lack = a.blocks_per_page * kFp4Rows - a.page_len;
+    int keys = nblk * kFp4Rows - (last - first) * lack;
+    if (whole) keys -= last == a.n_pages - 1 ? (a.total_blocks - last * a.blocks_per_page) * kFp4Rows - a.last_page_len : lack;
+    return keys;
+  };
 
   if (warp >= kFirstUnpackWarp) {
-    // =========================== dequantising warps ===========================
+    // =========================== unpacking warps: four take K, four V ===========================
     if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4UnpackRegs));
     // A thread takes half rows (sixteen bytes, 32 values) of rows tid / 2 and 64 further on: loads are consecutive, and eight threads
     // store to four rows and both their halves, which the swizzle puts into eight different 16-byte columns.
-    const int tid = threadIdx.x - 32 * kFirstUnpackWarp, row = tid >> 1;
-    const uint32_t to0 = sbase + L::tile_off + row * 128 + ((((tid & 1) * 4) ^ (row & 7)) << 4);
-    auto unpack = [&](const uint8_t* from, uint32_t to, int rows, int valid) {
+    const int v = (warp - kFirstUnpackWarp) >> 2, tid = (threadIdx.x - 32 * kFirstUnpackWarp) & 127, row = tid >> 1;
+    const uint32_t to0 = sbase + L::tile_off + v * kTileBytes + row * 128 + ((((tid & 1) * 4) ^ (row & 7)) << 4);
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, a.status)); };
+    Place at = first_place();
+    for (int j = 0, end = nblk; j < end; ++j) {
+      const int ps = j % kPackedStages, ts = j % kTileStages, rows = at.rows, valid = at.valid;
+      if (!wait(bar_packed_full(ps), (j / kPackedStages) & 1) || !wait(bar_tile_empty(ts, v), ((j / kTileStages) & 1) ^ 1u)) break;
+      const uint8_t* from = smem + L::packed_off + (ps * 2 + v) * kPackedBytes;
       uint4 w[2];
       uint32_t scales[2];
 #pragma unroll
@@ -199,27 +234,16 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           uint32_t p[4];
           fp4_unpack8(words[e], p);
           const uint32_t s = e < 2 ? s0 : s1;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((to ^ (e << 4)) + u * 8192), "r"(half2_mul(p[0], s)), "r"(half2_mul(p[1], s)),
-                       "r"(half2_mul(p[2], s)), "r"(half2_mul(p[3], s))
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(((to0 + ts * 2 * kTileBytes) ^ (e << 4)) + u * 8192), "r"(half2_mul(p[0], s)),
+                       "r"(half2_mul(p[1], s)), "r"(half2_mul(p[2], s)), "r"(half2_mul(p[3], s))
                        : "memory");
         }
       }
+      if (v == 0 && tid == 0) *reinterpret_cast<volatile int*>(smem + L::valid_off + 4 * (j % (2 * kTileStages))) = valid;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-    };
-    auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, cta_abort, a.status)); };
-    Place at = first_place();
-    for (int j = 0, end = nblk; j < end; ++j) {
-      const int ps = j % kPackedStages, ts = j % kTileStages, rows = rows_of(at), valid = valid_of(at);
-      const uint8_t* from = smem + L::packed_off + ps * 2 * kPackedBytes;
-      const uint32_t to = to0 + ts * 2 * kTileBytes, empty = ((j / kTileStages) & 1) ^ 1u;
-      if (!wait(bar_packed_full(ps), (j / kPackedStages) & 1) || !wait(bar_tile_empty(ts, 0), empty)) break;
-      unpack(from, to, rows, valid);
-      if (lane == 0) mbar_arrive(bar_tile_full(ts, 0));
-      if (!wait(bar_tile_empty(ts, 1), empty)) break;
-      unpack(from + kPackedBytes, to + kTileBytes, rows, valid);
       if (lane == 0) {
-        mbar_arrive(bar_tile_full(ts, 1));
+        mbar_arrive(bar_tile_full(ts, v));
         mbar_arrive(bar_packed_empty(ps));
       }
       advance(at);
@@ -235,7 +259,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       mbar_arrive_expect_tx(bar_q_full(), QT * kTileBytes);
       for (int t = 0; t < QT; ++t) tma_load_4d(sbase + L::q_off + t * kTileBytes, &tm_q, bar_q_full(), 0, h, (qg * QT + t) * kTileM, 0);
       int cur = -1;
-      const uint8_t* base = nullptr;
+      const uint8_t* from = nullptr;
       Place at = first_place();
       for (int j = 0, end = nblk; j < end; ++j) {
         if (at.page != cur) {
@@ -246,19 +270,20 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
             *cta_abort = 1;
             break;
           }
-          base = a.pool + (static_cast<int64_t>(page) * 2 * a.heads + h) * a.head_bytes;
+          from = a.pool + (static_cast<int64_t>(page) * 2 * a.heads + h) * a.head_bytes + static_cast<int64_t>(blocks_of(cur) - at.left) * kPackedBytes;
         }
         const int ps = j % kPackedStages;
         if (!mbar_wait(bar_packed_empty(ps), ((j / kPackedStages) & 1) ^ 1u, cta_abort, a.status)) break;
-        const uint32_t bytes = rows_of(at) * kFp4RowBytes<64>, to = sbase + L::packed_off + ps * 2 * kPackedBytes;
-        const uint8_t* from = base + static_cast<int64_t>(at.block) * kPackedBytes;
+        const uint32_t bytes = at.rows * kFp4RowBytes<64>, to = sbase + L::packed_off + ps * 2 * kPackedBytes;
         mbar_arrive_expect_tx(bar_packed_full(ps), 2 * bytes);
         bulk_load(to, from, bytes, bar_packed_full(ps));
         bulk_load(to + kPackedBytes, from + a.heads * a.head_bytes, bytes, bar_packed_full(ps));
+        from += kPackedBytes;
         advance(at);
         if (j + 1 == nblk && again()) {
           end = 2 * nblk;
           at = first_place();
+          cur = -1;
         }
       }
     }
@@ -274,6 +299,10 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
         const uint64_t bd = smem_desc(sbase + L::tile_off + s * 2 * kTileBytes, 16, 1024);
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_ss(lead, tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS16, k > 0);
+        if constexpr (kFold) {
+          const uint64_t xd = smem_desc(sbase + L::x_off, 16, 1024);
+          umma_ss(lead, tmem_base + t * 128, xd + 2 * t, xd + 4, kIdescS16, 1u);
+        }
       };
       auto issue_pv = [&](int s, int half, uint32_t accumulate) {
         const uint64_t bd = smem_desc(sbase + L::tile_off + (2 * s + 1) * kTileBytes, 16, 1024);
@@ -346,73 +375,87 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     constexpr uint32_t kPairSlot = QT * 2 * 128 * 4;
 
     // ---- once per CTA: the Q row in half precision, its factor and its fixed reference ----
+    // Normalised: times the power of two that puts its largest value into [2^14, 2^15): bf16 queries lose nothing that an fp32 sum would keep, and
+    // the row's factor in front of the exponential undoes it.  Folded: times scale * log2(e), where the reference holds and the row's values
+    // lie well inside the range of half precision.
     float* factor = reinterpret_cast<float*>(smem + L::factor_off) + t * 128 + row;
     float* reference = reinterpret_cast<float*>(smem + L::ref_off) + t * 128 + row;
-    if (half == 0) {
-      ok = wait_v(bar_q_full(), 0);
-      if (ok) {
-        const uint32_t q_row = sbase + L::q_off + t * kTileBytes + row * 128;
-        uint32_t w[32], top = 0;
+    auto softmax_sync = [&]() { asm volatile("bar.sync 15, %0;" ::"n"(256 * QT) : "memory"); };      // all softmax threads, also after a failed wait
+    {
+      const uint32_t q_row = sbase + L::q_off + t * kTileBytes + row * 128;
+      auto chunk = [&](int j) { return q_row + ((static_cast<uint32_t>(j) ^ (row & 7)) << 4); };
+      uint32_t top = 0;
+      if (half == 0) {
+        ok = wait_v(bar_q_full(), 0);
+        if (ok) {
+          float sq = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * j]), "=r"(w[4 * j + 1]), "=r"(w[4 * j + 2]), "=r"(w[4 * j + 3])
-                       : "r"(q_row + ((static_cast<uint32_t>(j) ^ (row & 7)) << 4)));
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(chunk(j)));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(w[4 * j + i] & 0x7fff0000u, (w[4 * j + i] & 0x7fffu) << 16));
-        }
-        // at most 2^126; 1 for a row of zeros or with a value that is not finite
-        const int up = top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
-        const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23), c = a.scale_log2 / f;
-        *factor = c;
-        float sq = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[4 * j + i] = pack_f16x2(__uint_as_float(w[4 * j + i] << 16) * f, __uint_as_float(w[4 * j + i] & 0xffff0000u) * f);
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[4 * j + i]));
-            sq = fmaf(x.x, x.x, fmaf(x.y, x.y, sq));
+            for (int i = 0; i < 4; ++i) {
+              const float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xffff0000u);
+              top = max(top, max(fp4_abs_bits(lo), fp4_abs_bits(hi)));
+              sq = fmaf(lo, lo, fmaf(hi, hi, sq));
+            }
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_row + ((static_cast<uint32_t>(j) ^ (row & 7)) << 4)), "r"(w[4 * j]),
-                       "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                       : "memory");
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (a.key_norm_max != nullptr) {
-          const float ref = sqrtf(sq) * __ldg(a.key_norm_max + h) * c;
-          *reference = ref;
-          if (!(ref <= a.fixed_limit)) *cta_exact = 1;     // too loose, infinite or NaN
+          if (a.key_norm_max != nullptr) {
+            // rounded up: to an eighth, which half precision holds, and by more than what rounding adds to the row (2^-11 relative)
+            const float ref = ceilf(8.008f * sqrtf(sq) * __ldg(a.key_norm_max + h) * a.scale_log2) * 0.125f, largest = __uint_as_float(top) * a.scale_log2;
+            *reference = ref;
+            if (!(ref <= a.fixed_limit) || (kFold && top != 0 && !(largest >= 0x1p-8f && largest <= 0x1p15f))) *cta_exact = 1;     // NaN too
+          }
         }
       }
+      softmax_sync();
+      if (half == 0 && ok) {
+        const bool folded = kFold && *cta_exact == 0;
+        // at most 2^64; 1 for a row of zeros or with a value that is not finite
+        const int up = top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 64);
+        const float f = folded ? a.scale_log2 : __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        *factor = folded ? 1.f : a.scale_log2 / f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(chunk(j)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk(j)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        if constexpr (kFold) {
+          const uint32_t x_row = sbase + L::x_off + row * 128;
+          auto st_chunk = [&](int j, uint32_t first) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %2, %2};" ::"r"(x_row + ((static_cast<uint32_t>(j) ^ (row & 7)) << 4)), "r"(first), "r"(0u) : "memory");
+          };
+          st_chunk(2 * t, folded ? pack_f16x2(kFixedShift - *reference, 0.f) : 0u);
+          st_chunk(2 * t + 1, 0u);
+          if (t == 0) {
+            st_chunk(4, 0x3c00u);
+            st_chunk(5, 0u);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_q_ready());
+      }
     }
-    auto softmax_sync = [&]() { asm volatile("bar.sync 15, %0;" ::"n"(256 * QT) : "memory"); };      // all softmax threads, also after a failed wait
-    softmax_sync();
     const bool fixed = *cta_exact == 0;
-    if (lane == 0) {
-      if (half == 0 && ok) mbar_arrive(bar_q_ready());
-      if (!fixed) mbar_arrive(bar_verdict());
-    }
+    if (!fixed && lane == 0) mbar_arrive(bar_verdict());
+    pair_sync();                                           // the factor of the row
     const float c = *factor;
     float m = -INFINITY, l = 0.f;                          // m: reference maximum (units of S); l: sum over this half
 
-    int pi, left;
-    auto rewind = [&]() {
-      pi = g0 / a.blocks_per_page;
-      left = blocks_of(pi) - (g0 - pi * a.blocks_per_page);
-    };
-    auto tail_valid = [&]() -> int {
-      const int valid = (pi == a.n_pages - 1 ? a.last_page_len : a.page_len) - (blocks_of(pi) - 1) * kBlockN - 64 * half;
-      left = blocks_of(++pi);
-      return valid;
-    };
-    // P = exp2(S c + shift) of 64 logits as half-precision pairs, and their sum, software-pipelined over pairs as in gct_attn_kernel.  kNum of
+    // P = exp2(S c + shift) of some logits as half-precision pairs, and their sum, software-pipelined over pairs as in gct_attn_kernel.  kNum of
     // kDen pairs take the FMA pipe; kBelow: exponents may lie below -126.
-    auto sweep = [&](uint32_t (&s)[64], uint32_t (&pk)[32], float shift, auto below, auto num, auto den) -> float {
+    auto sweep = [&](auto& s, auto& pk, float shift, auto below, auto num, auto den) -> float {
+      constexpr int kPairs = sizeof(pk) / sizeof(pk[0]);
       constexpr bool kBelow = decltype(below)::value;
       constexpr int kNum = decltype(num)::value, kDen = decltype(den)::value;
       const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
       float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
       auto pair_ffma = [&](int q) {
+        if constexpr (!kBelow && kFold) return;            // S is the exponent
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), c2, shift2);
         s[2 * q] = __float_as_uint(x.x);
         s[2 * q + 1] = __float_as_uint(x.y);
@@ -436,77 +479,77 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
 #pragma unroll
       for (int q = 0; q < kFfmaAhead; ++q) pair_ffma(q);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        if (q + kFfmaAhead < 32) pair_ffma(q + kFfmaAhead);
+      for (int q = 0; q < kPairs; ++q) {
+        if (q + kFfmaAhead < kPairs) pair_ffma(q + kFfmaAhead);
         pair_exp(q);
         if (q >= kSumLag) pair_sum(q - kSumLag);
       }
 #pragma unroll
-      for (int q = 32 - kSumLag; q < 32; ++q) pair_sum(q);
+      for (int q = kPairs - kSumLag; q < kPairs; ++q) pair_sum(q);
       return (acc0.x + acc0.y) + (acc1.x + acc1.y);
     };
     using std::integral_constant;
     using Yes = std::true_type;
     using No = std::false_type;
-    // S of block j in registers, the tile free for the next
-    auto load_s = [&](int j, uint32_t (&s)[64]) -> bool {
-      if (!wait_u(bar_s_full(t), j & 1)) return false;
-      tc_fence_after();
-      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+    auto load_s = [&](int ch, int valid, uint32_t hidden, uint32_t (&s)[32]) {       // 32 columns of this thread's half; `valid` of the 64 count
+      tmem_ld32(s_addr + 32 * ch, s);
       tmem_wait_ld();
+      if (valid < 64) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (32 * ch + i >= valid) s[i] = hidden;
+      }
+    };
+    auto s_taken = [&]() {                                 // the tensor core may overwrite S with the next block
       tc_fence_before();
       __syncwarp();
       mbar_arrive_elected(lead, bar_s_empty(t));
-      return true;
     };
-    auto store_p = [&](const uint32_t (&pk)[32]) {
-      tmem_st32(p_addr, pk);
+    auto p_stored = [&]() {
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       mbar_arrive_elected(lead, bar_p_full(t, half));
     };
-    auto mask = [&](uint32_t (&s)[64], int valid) {
-#pragma unroll
-      for (int i = 0; i < 64; ++i)
-        if (i >= valid) s[i] = 0xff800000u;
-    };
-
+    auto valid_rows = [&](int j) { return *reinterpret_cast<volatile int*>(smem + L::valid_off + 4 * (j % (2 * kTileStages))); };
     // ---- fixed reference: |q| max|k| bounds every exponent of the row (Cauchy-Schwarz); no maximum, no exchange, no rescaling ----
     // Weights are exp2(x - ref + 15), at most 2^15.  Half precision holds them to 2^-25 at least, so over n keys at most n 2^-25 of the sum is lost
     // to rounding small ones; a row whose sum is at least n 2^-15 has lost less than 2^-10 of it.  A CTA with a row below that goes through its
     // range again with the running maximum.
     bool held = false;
-    rewind();
     if (fixed) {
-      const float shift = kFixedShift - *reference;
-      int keys = nblk * kBlockN;
+      const float shift = kFold ? 0.f : kFixedShift - *reference;
+      const uint32_t hidden = __float_as_uint(kFold ? -100.f : (-100.f - shift) / c);      // weighs 2^-100
       for (int j = 0; ok && j < nblk; ++j) {
-        uint32_t s[64], pk[32];
-        if (!(ok = load_s(j, s))) break;
-        int valid = 64;
-        if (--left == 0) {
-          valid = tail_valid();
-          keys -= kBlockN - min(valid + 64 * half, kBlockN);
+        if (!(ok = wait_u(bar_s_full(t), j & 1))) break;
+        tc_fence_after();
+        const int valid = valid_rows(j) - 64 * half;
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t s[32], pk[16];
+          tmem_ld32(s_addr + 32 * ch, s);
+          tmem_wait_ld();
+          if (ch == 1) s_taken();
+          if (valid < 64) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * ch + i >= valid) s[i] = hidden;
+          }
+          l += sweep(s, pk, shift, No(), integral_constant<int, kFixedNum>(), integral_constant<int, kFixedDen>());
+          if (ch == 0 && j > 0) {                          // P is free once the product of the block before has read it
+            if (!(ok = wait_u(bar_pv_full(t, half), (j - 1) & 1))) break;
+            tc_fence_after();
+          }
+          tmem_st16(p_addr + 16 * ch, pk);
         }
-        if (valid < 64) {
-          mask(s, valid);
-          l += sweep(s, pk, shift, Yes(), integral_constant<int, 0>(), integral_constant<int, 1>());
-        } else {
-          l += sweep(s, pk, shift, No(), integral_constant<int, 1>(), integral_constant<int, 4>());
-        }
-        if (j > 0) {
-          if (!(ok = wait_u(bar_pv_full(t, half), (j - 1) & 1))) break;
-          tc_fence_after();
-        }
-        store_p(pk);
+        if (!ok) break;
+        p_stored();
       }
       __syncwarp();
       if (ok && nblk > 0) ok = wait_v(bar_pv_full(t, 1), (nblk - 1) & 1);
       const float other = pair_exchange(l, 0);
       l = half == 0 ? l + other : other + l;
-      if (ok && !(l >= static_cast<float>(keys) * 0x1p-15f)) *cta_redo = 1;
+      if (ok && !(l >= static_cast<float>(keys_of_range()) * 0x1p-15f)) *cta_redo = 1;
       softmax_sync();
       held = *cta_redo == 0;
       if (lane == 0) mbar_arrive(bar_verdict());
@@ -514,7 +557,6 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
         m = *reference;
       } else {
         l = 0.f;
-        rewind();
       }
     }
     // ---- running maximum ----
@@ -522,18 +564,22 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       const int first = fixed ? nblk : 0;
       int met = 0;
       for (int j = first; ok && j < first + nblk; ++j) {
-        uint32_t s[64], pk[32];
-        if (!(ok = load_s(j, s))) break;
-        if (--left == 0) {
-          const int valid = tail_valid();
-          if (valid < 64) mask(s, valid);
+        if (!(ok = wait_u(bar_s_full(t), j & 1))) break;
+        tc_fence_after();
+        const int valid = valid_rows(j) - 64 * half;
+        // S is read twice: the maximum, then the weights
+        uint32_t s[32], pk[16];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          load_s(ch, valid, 0xff800000u, s);
+          float mxc[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mxc[i] = __uint_as_float(s[i]);
+#pragma unroll
+          for (int i = 4; i < 32; i += 2) mxc[(i >> 1) & 3] = max3(mxc[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          mx = fmaxf(mx, fmaxf(fmaxf(mxc[0], mxc[1]), fmaxf(mxc[2], mxc[3])));
         }
-        float mxc[4];
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) mxc[ch] = __uint_as_float(s[ch]);
-#pragma unroll
-        for (int i = 4; i < 64; i += 2) mxc[(i >> 1) & 3] = max3(mxc[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        float mx = fmaxf(fmaxf(mxc[0], mxc[1]), fmaxf(mxc[2], mxc[3]));
         mx = fmaxf(mx, pair_exchange(mx, ((met + 1) & 1) * kPairSlot));
         ++met;
         float alpha = 1.f;
@@ -541,28 +587,43 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
           alpha = fast_exp2((m - mx) * c);
           m = mx;
         }
-        const float sum = sweep(s, pk, kFp4Shift - m * c, Yes(), integral_constant<int, QT == 2 ? 2 : 1>(), integral_constant<int, QT == 2 ? 7 : 3>());
-        l = fmaf(l, alpha, sum);
-        if (j > first) {
-          if (!(ok = wait_u(bar_pv_full(t, 1), (j - 1) & 1))) break;
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, alpha != 1.f)) {
-            uint32_t ob[32];
-            tmem_ld32(o_addr, ob);
-            tmem_wait_ld();
+        // exponents so large that rounding m * c would move them: the maximum is taken off first
+        const float base = m * c;
+        const bool huge = __any_sync(0xffffffffu, fabsf(base) > 65536.f);
+        l *= alpha;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * alpha);
-            tmem_st32(o_addr, ob);
+        for (int ch = 0; ch < 2; ++ch) {
+          load_s(ch, valid, 0xff800000u, s);
+          if (ch == 1) s_taken();
+          if (huge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - m);
           }
+          l += sweep(s, pk, kFp4Shift - (huge ? 0.f : base), Yes(), integral_constant<int, QT == 2 ? 2 : 1>(), integral_constant<int, QT == 2 ? 7 : 3>());
+          if (ch == 0 && j > first) {
+            if (!(ok = wait_u(bar_pv_full(t, 1), (j - 1) & 1))) break;
+            tc_fence_after();
+            if (__any_sync(0xffffffffu, alpha != 1.f)) {
+              uint32_t ob[32];
+              tmem_ld32(o_addr, ob);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(__uint_as_float(ob[i]) * alpha);
+              tmem_st32(o_addr, ob);
+            }
+          }
+          tmem_st16(p_addr + 16 * ch, pk);
         }
-        store_p(pk);
+        if (!ok) break;
+        p_stored();
       }
       __syncwarp();
       for (; met < nblk; ++met) pair_sync();
       if (ok && nblk > 0) ok = wait_v(bar_pv_full(t, 1), (first + nblk - 1) & 1);
       const float other = pair_exchange(l, ((nblk + 1) & 1) * kPairSlot);
       l = half == 0 ? l + other : other + l;
-      m = m * c + (kFixedShift - kFp4Shift);               // as below: the exponent that weighs 2^kFixedShift
+      // as above: the exponent that weighs 2^kFixedShift; a first pass has left its reference folded into S
+      m = m * c + (kFixedShift - kFp4Shift) - (kFold && fixed ? kFixedShift - *reference : 0.f);
     }
 
     // ---- epilogue: O / l ----
@@ -620,20 +681,27 @@ int prepare_device() {
   if (dev < 0 || dev >= 64) return fail(GCT_ERR_INVALID, "attention: device ordinal out of range");
   std::lock_guard<std::mutex> lock(g_fp4_mutex);
   if (g_fp4_ready[dev]) return GCT_OK;
-  GCT_CUDA_CHECK(cudaFuncSetAttribute(gct_attn_fp4_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp4Smem<1>::total + 1024));
-  GCT_CUDA_CHECK(cudaFuncSetAttribute(gct_attn_fp4_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp4Smem<2>::total + 1024));
   // setmaxnreg hands out no more registers than the CTA was launched with and waits for ever for the rest: never launch such a build
-  cudaFuncAttributes attr;
-  GCT_CUDA_CHECK(cudaFuncGetAttributes(&attr, gct_attn_fp4_kernel<2>));
-  if (attr.numRegs * kFp4Threads<2> < 512 * kFp4SoftmaxRegs + 128 * kFp4ControlRegs + 128 * kFp4UnpackRegs)
-    return fail(GCT_ERR_INVALID, "attention: the kernel was built with fewer registers than its warpgroups share");
+  auto prepare = [](auto kernel, int smem, int pool) -> int {
+    GCT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes attr;
+    GCT_CUDA_CHECK(cudaFuncGetAttributes(&attr, kernel));
+    return attr.numRegs < pool ? fail(GCT_ERR_INVALID, "attention: the kernel was built with fewer registers than its warpgroups share") : GCT_OK;
+  };
+  constexpr int kPool = (512 * kFp4SoftmaxRegs + 128 * kFp4ControlRegs + 256 * kFp4UnpackRegs) / kFp4Threads<2>;
+  int rc = prepare(gct_attn_fp4_kernel<2, true>, Fp4Smem<2>::total + 1024, kPool);
+  if (rc == GCT_OK) rc = prepare(gct_attn_fp4_kernel<2, false>, Fp4Smem<2>::total + 1024, kPool);
+  if (rc == GCT_OK) rc = prepare(gct_attn_fp4_kernel<1, true>, Fp4Smem<1>::total + 1024, 0);
+  if (rc == GCT_OK) rc = prepare(gct_attn_fp4_kernel<1, false>, Fp4Smem<1>::total + 1024, 0);
+  if (rc != GCT_OK) return rc;
   g_fp4_ready[dev] = true;
   return GCT_OK;
 }
 
 }  // namespace
 
-int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, const int32_t* page_ids, cudaStream_t stream) {
+int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, const int32_t* page_ids, bool exact_logits,
+                         cudaStream_t stream) {
   if (a.n_q <= 0 || a.heads <= 0 || a.batch != 1 || a.n_pages <= 0 || a.page_len <= 0 || a.last_page_len <= 0 || a.last_page_len > a.page_len ||
       pool == nullptr || (a.page_table == nullptr && page_ids == nullptr) || a.status == nullptr || (a.q_tiles_per_cta != 1 && a.q_tiles_per_cta != 2))
     return fail(GCT_ERR_INVALID, "attention: bad shape");
@@ -681,10 +749,11 @@ int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layo
     std::copy(page_ids, page_ids + a.n_pages, pages.id);
     k.page_table = nullptr;
   }
+  auto launch = [&](auto kernel, int threads, int smem) { return launch_pdl(kernel, g, dim3(threads), smem, stream, a.tm_q, k, pages); };
   if (a.q_tiles_per_cta == 2)
-    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<2>, g, dim3(kFp4Threads<2>), Fp4Smem<2>::total + 1024, stream, a.tm_q, k, pages));
+    GCT_CUDA_CHECK(launch(exact_logits ? gct_attn_fp4_kernel<2, false> : gct_attn_fp4_kernel<2, true>, kFp4Threads<2>, Fp4Smem<2>::total + 1024));
   else
-    GCT_CUDA_CHECK(launch_pdl(gct_attn_fp4_kernel<1>, g, dim3(kFp4Threads<1>), Fp4Smem<1>::total + 1024, stream, a.tm_q, k, pages));
+    GCT_CUDA_CHECK(launch(exact_logits ? gct_attn_fp4_kernel<1, false> : gct_attn_fp4_kernel<1, true>, kFp4Threads<1>, Fp4Smem<1>::total + 1024));
   return GCT_OK;
 }
 

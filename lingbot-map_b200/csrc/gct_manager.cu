@@ -779,9 +779,9 @@ static int timed(gct_mgr* m, cudaStream_t stream, F&& launch) {
   }
   return rc;
 }
-static int timed_attention(gct_mgr* m, int block, const AttnLaunch& a, cudaStream_t stream) {
+static int timed_attention(gct_mgr* m, int block, const AttnLaunch& a, bool with_lse, cudaStream_t stream) {
   return timed(m, stream, [&] {
-    return m->fp4 ? launch_attention_fp4(a, m->pools4[block], m->fp4_page, m->geo.max_num_pages, m->plan_ids.empty() ? nullptr : m->plan_ids.data(), stream)
+    return m->fp4 ? launch_attention_fp4(a, m->pools4[block], m->fp4_page, m->geo.max_num_pages, m->plan_ids.empty() ? nullptr : m->plan_ids.data(), with_lse, stream)
                   : launch_attention(a, stream);
   });
 }
@@ -891,19 +891,19 @@ static int run_paged(gct_mgr* m, int block, const void* q_dev, int q_dtype, int 
     a.part_lse = m->part_lse;
     *splits_out = a.splits;
     m->launches += 1;
-    return timed_attention(m, block, a, stream);
+    return timed_attention(m, block, a, lse_dev != nullptr, stream);
   }
   if (a.splits == 1 && out_bf16 != nullptr && lse_dev == nullptr) {
     a.final_bf16 = true;
     a.out = out_bf16;
     m->launches += 1;
-    return timed_attention(m, block, a, stream);
+    return timed_attention(m, block, a, lse_dev != nullptr, stream);
   }
   a.final_bf16 = false;
   a.part_o = m->part_o;
   a.part_lse = m->part_lse;
   // partial rows are laid out with n_q rows per split
-  rc = timed_attention(m, block, a, stream);
+  rc = timed_attention(m, block, a, lse_dev != nullptr, stream);
   if (rc != GCT_OK) return rc;
   m->launches += 2;
   return launch_merge(m->part_o, m->part_lse, a.splits, rows, out_bf16, out_f32, lse_dev, stream);

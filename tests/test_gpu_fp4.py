@@ -233,6 +233,24 @@ def test_queries_of_any_magnitude(scale):
         assert (np.abs(out[i:i + 1] - want[i:i + 1]) <= tol).all(), i
 
 
+@pytest.mark.parametrize("with_lse", [False, True])
+@pytest.mark.parametrize("scale", [1e-30, 2.0 ** -12, 300.0, 2.0 ** 60])
+def test_query_tiles_of_any_magnitude(scale, with_lse):
+    """The same through the query tiles, whose CTAs fold scale and reference into the product only where all their rows allow it."""
+    rs = np.random.RandomState(2)
+    m, k, v = filled(60, 1, 5, rs)
+    q = bf(rs.standard_normal((40, 1, 64)) * np.where(np.arange(40) % 7 == 3, scale, np.where(np.arange(40) % 7 == 5, 0.0, 1.0))[:, None, None])
+    want, want_lse, weighted = F.attention(q, k, v)
+    got = m.compute_attention(0, dev(q, torch.bfloat16), return_lse=with_lse)
+    out = host(got[0] if with_lse else got)
+    assert np.isfinite(out).all()
+    for i in range(40):
+        spread = spread_of(q[i:i + 1], k)
+        assert (np.abs(out[i] - want[i]) <= bound_frame(len(k), spread, weighted[i], want[i])).all(), i
+        if with_lse:
+            assert np.abs(host(got[1])[i] - want_lse[i]).max() <= 2.0 ** -16 * spread + 2.0 ** -13 + len(k) * 2.0 ** -23 + 2.0 ** -22 * np.abs(want_lse[i]).max(), i
+
+
 def test_values_that_are_not_finite_stay_visible_and_hidden_ones_do_not_leak():
     rs = np.random.RandomState(7)
     T, H = 40, 2
