@@ -740,10 +740,10 @@ double list_schedule(int n_long, double len_long, int n_short, double len_short,
 }
 
 struct SplitPlanKey {
-  int n_q_tiles, heads_x_batch, total_blocks, num_sms, max_splits;
+  int n_q_tiles, heads_x_batch, total_blocks, num_sms, max_splits, uneven_max_blocks;
   bool operator==(const SplitPlanKey& o) const {
     return n_q_tiles == o.n_q_tiles && heads_x_batch == o.heads_x_batch && total_blocks == o.total_blocks &&
-           num_sms == o.num_sms && max_splits == o.max_splits;
+           num_sms == o.num_sms && max_splits == o.max_splits && uneven_max_blocks == o.uneven_max_blocks;
   }
 };
 struct SplitPlan {
@@ -753,7 +753,7 @@ struct SplitPlan {
 }  // namespace
 
 void choose_attention_config(int n_q_tiles, int heads_x_batch, int total_blocks, int num_sms, int max_splits,
-                             int* q_tiles_per_cta, int* splits, int* split_len) {
+                             int* q_tiles_per_cta, int* splits, int* split_len, int uneven_max_blocks) {
   // Cost model in units of "one KV block for one CTA": a CTA with two query tiles takes about as long
   // per block as one with a single tile takes for 0.6 blocks-worth of its pair; every wave of CTAs pays for
   // its prologue and epilogue, and a split result needs the merge kernel afterwards (a launch
@@ -779,12 +779,11 @@ void choose_attention_config(int n_q_tiles, int heads_x_batch, int total_blocks,
   auto fixed = [paged](int qt, bool one_wave) { return !paged ? 2.0 : one_wave ? (qt == 2 ? 5.0 : 4.0) : (qt == 2 ? 15.0 : 9.0); };
   // Long ranges + a short one fill the SMs that equal ranges leave idle (the table above).  The line at a thousand blocks was drawn with
   // one thread per row, where nine long ranges and a short one were 0.6 % slower than nine equal ones at 1057 blocks; two long ranges
-  // and a short one, 2.5 % faster there now, were not measured then.
-  constexpr int kUnevenMaxBlocks = 1000;
+  // and a short one, 2.5 % faster there now, were not measured then.  The 4-bit cache's calls set it higher.
   // the plan of the previous call with the same arguments (a frame asks 24 times for the same one)
-  static thread_local SplitPlanKey last_key = {-1, -1, -1, -1, -1};
+  static thread_local SplitPlanKey last_key = {-1, -1, -1, -1, -1, -1};
   static thread_local SplitPlan last_plan = {1, 1, 0};
-  const SplitPlanKey key = {n_q_tiles, heads_x_batch, total_blocks, num_sms, max_splits};
+  const SplitPlanKey key = {n_q_tiles, heads_x_batch, total_blocks, num_sms, max_splits, uneven_max_blocks};
   if (split_len != nullptr && key == last_key) {
     *q_tiles_per_cta = last_plan.qt;
     *splits = last_plan.splits;
@@ -811,7 +810,7 @@ void choose_attention_config(int n_q_tiles, int heads_x_batch, int total_blocks,
       }
     }
     // s - 1 long ranges and a short one, the short CTAs last: try a few lengths of the short range per s
-    if (!paged || total_blocks > kUnevenMaxBlocks || items * 2 > 4096) continue;
+    if (!paged || total_blocks > uneven_max_blocks || items * 2 > 4096) continue;
     for (int s = 2; s <= smax; ++s) {
       const int even = (total_blocks + s - 1) / s;
       for (int step = 1; step <= 12; ++step) {

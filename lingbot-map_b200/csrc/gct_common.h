@@ -106,9 +106,9 @@ int make_tensor_map(CUtensorMap* out, const void* base, int heads, int64_t token
 // Pick (q_tiles_per_cta, splits) for a problem: n_q_tiles query tiles of 128 rows per (head,batch),
 // total_blocks KV blocks, on num_sms SMs, with at most max_splits partial results.  With split_len != nullptr the
 // plan may also be splits - 1 long ranges plus one short one (AttnLaunch::split_len), which fills the SMs that a whole
-// number of equal ranges leaves idle; *split_len = 0 when equal ranges are at least as good.
+// number of equal ranges leaves idle (calls of up to uneven_max_blocks KV blocks); *split_len = 0 when equal ranges are at least as good.
 void choose_attention_config(int n_q_tiles, int heads_x_batch, int total_blocks, int num_sms, int max_splits,
-                             int* q_tiles_per_cta, int* splits, int* split_len = nullptr);
+                             int* q_tiles_per_cta, int* splits, int* split_len = nullptr, int uneven_max_blocks = 1000);
 
 // Frustum culling with the camera on the host (packed) or, to spare two synchronising copies, in device memory with the given
 // strides (row and column of R, step of t).

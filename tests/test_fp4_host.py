@@ -139,3 +139,22 @@ def test_c_entry_points_refuse_bad_arguments():
     read = lambda first, rows, cap: lib.gct_decode_read_fp4(one, one, first, rows, cap, 2, 64, one, one, one, one, None)
     assert read(-1, 1, 128) == _lib.ERR_INVALID and read(0, 129, 128) == _lib.ERR_INVALID and read(120, 9, 128) == _lib.ERR_INVALID
     assert read(128, 0, 128) == _lib.GCT_OK
+
+
+def test_camera_head_conversion_keeps_the_width():
+    """convert_camera_head marks the layers; the caches are made with the first token that they see."""
+    from lingbot_map_b200.camera import convert_camera_head
+
+    class Attn(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.qkv, self.gate_proj = torch.nn.Linear(2, 2), None
+
+    head = torch.nn.Module()
+    head.trunk = torch.nn.ModuleList([torch.nn.Module() for _ in range(3)])
+    for blk in head.trunk:
+        blk.attn = Attn()
+    assert convert_camera_head(head, 4) == 3 and all(b.attn.b200_kv_bits == 4 for b in head.trunk)
+    assert convert_camera_head(head) == 0                   # converted already
+    with pytest.raises(ValueError):
+        convert_camera_head(head, 8)

@@ -522,3 +522,85 @@ def test_stream_of_frames_on_another_stream():
                 m.rollback_last_frame(0)
                 m._defer_eviction = False
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_blocks_stream_on_a_4bit_cache(dtype):
+    """Two global blocks through a scale pass, streamed frames and a frame that is no keyframe.  The native layer and the modules fill the cache
+    with the same bytes and agree in their outputs; what is cached is the quantisation of what the bf16 cache holds, layer by layer."""
+    from test_gpu_blocks import rope3d_pos
+    pph, ppw, scale, dim, H = 5, 7, 2, 128, 2
+    T = NS + pph * ppw
+    torch.manual_seed(3)
+    blocks = [P.B200Block(dim=dim, num_heads=H, init_values=0.5, qk_norm=True, rope=object(), kv_cache_sliding_window=2, kv_cache_scale_frames=scale).to(DEV).to(dtype)
+              for _ in range(2)]
+    make = lambda bits: P.B200KVCacheManager(2, 30, T, H, 64, device=DEV, scale_frames=scale, sliding_window=2, max_total_frames=40, kv_bits=bits)
+    xs = [torch.randn(1, scale * T, dim, device=DEV, dtype=dtype)] + [torch.randn(1, T, dim, device=DEV, dtype=dtype) for _ in range(6)]
+
+    def run(mgr, native, one_layer=False):
+        outs = []
+        for f, x in enumerate(xs):
+            frames = scale if f == 0 else 1
+            mgr._skip_append = f == 4
+            kw = dict(num_patches=T - NS, num_special=NS, enable_3d_rope=True, num_frames=frames, kv_cache=mgr,
+                      pos=rope3d_pos(0 if f == 0 else scale + f - 1, frames, pph, ppw, NS))
+            with torch.set_grad_enabled(not native), torch.autocast("cuda", dtype=torch.bfloat16):      # gradients on: the modules
+                y = x
+                for b, blk in enumerate(blocks[:1] if one_layer else blocks):
+                    y = blk(y, global_idx=b, **kw)
+            outs.append(y.detach())
+        return outs
+
+    slim, slim2, wide = make(4), make(4), make(16)
+    got, want = run(slim, True), run(slim2, False)
+    # the first block's inputs are the same both ways: the same bytes
+    assert torch.equal(slim.kv_caches[0], slim2.kv_caches[0]) or dtype == torch.float32
+    for a, b in zip(got, want):
+        assert a.shape == b.shape and float((a.float() - b.float()).abs().max()) <= 3 * 2 ** -7 * float(b.float().abs().max())
+    run(wide, True, one_layer=True)
+    slim3 = make(4)
+    run(slim3, True, one_layer=True)
+    for a, b in zip(wide._gather_kv(0), slim3._gather_kv(0)):
+        assert (host(b) == F.roundtrip(host(a))).all()
+    assert slim.device_status() == slim2.device_status() == 0
+
+
+def test_many_blocks_and_heads_track_no_key_norms():
+    """A geometry whose key norms do not fit the workspace header: every call runs with the running maximum."""
+    m = P.B200KVCacheManager(100, 21, 14, 10, 64, device=DEV, scale_frames=1, sliding_window=1, max_total_frames=4, kv_bits=4)
+    rs = np.random.RandomState(6)
+    k, v, q = (rs.standard_normal((14, 10, 64)) for _ in range(3))
+    for b in (0, 99):
+        m.append_frame(b, dev(k), dev(v))
+        m.append_frame(b, dev(v), dev(k))
+    q = bf(q)
+    for b in (0, 99):
+        kk, vv = (host(x) for x in m._gather_kv(b))
+        for n_q in (5, 14):
+            want, _, weighted = F.attention(q[:n_q], kk, vv)
+            out = host(m.compute_attention(b, dev(q[:n_q], torch.bfloat16)))
+            assert (np.abs(out - want) <= bound_frame(len(kk), spread_of(q[:n_q], kk), weighted, want)).all()
+    with pytest.raises(RuntimeError):
+        m.key_norm_max
+
+
+def test_attention_captured_into_a_graph():
+    """A plan of few pages is a kernel argument: append apart, a whole attention call can be captured and replayed on new queries."""
+    rs = np.random.RandomState(8)
+    m, k, v = filled(60, 2, 6, rs)
+    for n_q in (3, 60):
+        q = torch.zeros(n_q, 2, 64, device=DEV, dtype=torch.bfloat16)
+        m.compute_attention(0, q)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = m.compute_attention(0, q)
+        for seed in range(3):
+            x = bf(np.random.RandomState(seed).standard_normal((n_q, 2, 64)))
+            q.copy_(dev(x, torch.bfloat16))
+            g.replay()
+            torch.cuda.synchronize()
+            want, _, weighted = F.attention(x, k, v)
+            assert (np.abs(host(out) - want) <= bound_frame(len(k), spread_of(x, k), weighted, want)).all()
+    assert m.device_status() == 0
