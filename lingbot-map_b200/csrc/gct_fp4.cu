@@ -167,6 +167,10 @@ struct RowsSmem {
   static_assert(8 * D / 4 * 32 <= new_off && 128 * 32 <= new_off, "lane sums do not fit the ring");
 };
 
+// Floats of a key range's partial result of a query: sums, maximum, sum of weights, and two that make it a multiple of sixteen bytes.
+template <int D>
+constexpr int kRowsRecord = D + 4;
+
 struct RowsArgs {
   const void* q;
   int q_f32, q_round_bf16, n_q, heads, groups, splits;
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kerne
     if (a.lse != nullptr && d == 0) a.lse[row] = (mx + log2f(den) - kWeightShift) * 0.6931471805599453f;
   };
   const size_t item = static_cast<size_t>(h) * a.groups + group;
-  constexpr int kRecord = D + 2;
+  constexpr int kRecord = kRowsRecord<D>;
   for (int e = threadIdx.x; e < rows_here * D; e += kRowsThreads) {
     const int i = e / D, d = e % D;
     float mx = -INFINITY;
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kerne
   // maximum among them, then they are joined in order.  Maxima and sums come in one trip.
   float4* lane_sum = reinterpret_cast<float4*>(smem);
   const float* recs = a.part + item * a.splits * 8 * kRecord;
-  constexpr int kCols = D / 4, kAhead = 5;
+  constexpr int kCols = D / 4, kAhead = 9;                 // ranges in flight: with five, eight queries at D = 128 took 4 us longer
   const int items = rows_here * kCols;
   int lanes = 1;
   while (2 * lanes * items <= 128) lanes *= 2;
@@ -604,14 +608,14 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kerne
     float mx = -INFINITY, den = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int r0 = ln; r0 < a.splits; r0 += kAhead * lanes) {
-      float2 lo[kAhead], hi[kAhead], ml[kAhead];
+      float4 o[kAhead];
+      float2 ml[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int r = r0 + u * lanes;
         const float* rec = recs + (r * 8 + i) * kRecord;
         ml[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + D)) : make_float2(-INFINITY, 0.f);
-        lo[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + 4 * col)) : make_float2(0.f, 0.f);
-        hi[u] = r < a.splits ? __ldcg(reinterpret_cast<const float2*>(rec + 4 * col + 2)) : make_float2(0.f, 0.f);
+        o[u] = r < a.splits ? __ldcg(reinterpret_cast<const float4*>(rec + 4 * col)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float next = mx;
 #pragma unroll
@@ -627,10 +631,10 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kerne
       for (int u = 0; u < kAhead; ++u) {
         const float f = ml[u].x == mx ? 1.f : fast_exp2(ml[u].x - mx);
         den = fmaf(f, ml[u].y, den);
-        sum.x = fmaf(f, lo[u].x, sum.x);
-        sum.y = fmaf(f, lo[u].y, sum.y);
-        sum.z = fmaf(f, hi[u].x, sum.z);
-        sum.w = fmaf(f, hi[u].y, sum.w);
+        sum.x = fmaf(f, o[u].x, sum.x);
+        sum.y = fmaf(f, o[u].y, sum.y);
+        sum.z = fmaf(f, o[u].z, sum.z);
+        sum.w = fmaf(f, o[u].w, sum.w);
       }
     }
     lane_sum[2 * e] = sum;
@@ -686,7 +690,7 @@ int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, si
   if (blocks <= 1 || items > num_counters) return 1;
   const int64_t slots = static_cast<int64_t>(sms) * (head_dim == 64 ? kRowsCtas<64> : kRowsCtas<128>);
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / items, blocks));
-  splits = std::min<int64_t>(splits, static_cast<int64_t>(part_floats / (static_cast<size_t>(items) * 8 * (head_dim + 2))));
+  splits = std::min<int64_t>(splits, static_cast<int64_t>(part_floats / (static_cast<size_t>(items) * 8 * (head_dim == 64 ? kRowsRecord<64> : kRowsRecord<128>))));
   return static_cast<int>(std::max<int64_t>(splits, 1));
 }
 
@@ -796,7 +800,7 @@ constexpr size_t kDecodeStatusBytes = 256;
 constexpr int kDecodeCounters = 2048;
 // Counters and partial results of one wave of CTAs; calls with more (head, eight queries) items than counters take one key range.
 size_t decode_fp4_workspace(int head_dim) {
-  return kDecodeStatusBytes + kDecodeCounters * sizeof(int) + static_cast<size_t>(148 * (head_dim == 64 ? gct::kRowsCtas<64> : gct::kRowsCtas<128>)) * 8 * (head_dim + 2) * sizeof(float);
+  return kDecodeStatusBytes + kDecodeCounters * sizeof(int) + static_cast<size_t>(148 * (head_dim == 64 ? gct::kRowsCtas<64> : gct::kRowsCtas<128>)) * 8 * (head_dim == 64 ? gct::kRowsRecord<64> : gct::kRowsRecord<128>) * sizeof(float);
 }
 
 int check_decode_cache(const char* who, int heads, int head_dim, int capacity) {
