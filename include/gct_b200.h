@@ -160,7 +160,9 @@ int gct_mgr_free_list(const gct_mgr_t* m, int block, int which, int32_t* out, in
 
 /* The plan() half of compute_attention (flashinfer_cache.py:385-414): snapshot block 0's visible
  * table and upload it; valid for every block until the next plan.  page_begin/page_end select a
- * sub-range of the visible list (0, -1 = all) for KV-sharded execution. */
+ * sub-range of the visible list (0, -1 = all) for KV-sharded execution.
+ * A 4-bit cache's plan of at most 256 pages is not uploaded but passed to the kernels as an argument: an attention call captured into a
+ * graph attends to the pages that were planned when it was captured. */
 int gct_mgr_plan(gct_mgr_t* m, int page_begin, int page_end, void* stream);
 
 /* The run() half (flashinfer_cache.py:416-421): softmax(q k^T / 8) v over the planned pages of `block`.
@@ -282,7 +284,7 @@ int gct_decode_attention(const float* q_dev, const float* k_new_dev, const float
  * the fp32 rows; capacity is a multiple of 128, gct_decode_fp4_sizes gives the bytes of either cache.  n_new: any number of new tokens;
  * they are quantised before they are attended to, stored or not.  q, out and the arithmetic are fp32 (products of q and of the weights in
  * two half-precision parts: about 2^-21).  The workspace must be zero before the first call; its first word is a status word as
- * gct_mgr_device_status reports it. */
+ * gct_mgr_device_status reports it.  Calls that share a workspace are ordered among themselves. */
 int gct_decode_fp4_sizes(int heads, int head_dim, int capacity, size_t* cache_bytes_out, size_t* workspace_bytes_out);
 int gct_decode_attention_fp4(const float* q_dev, const float* k_new_dev, const float* v_new_dev, int n_new, uint8_t* cache_k_dev,
                              uint8_t* cache_v_dev, int cached, int capacity, int store, int heads, int head_dim, float* out_dev,

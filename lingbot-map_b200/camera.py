@@ -26,7 +26,9 @@ class DecodeCache:
     """K and V rows of one (refinement iteration, block) pair: [capacity, H, D] fp32, `count` rows valid.
 
     With kv_bits=4 the rows are held in 4-bit values with a scale for 16 of them (include/gct_b200.h, gct_decode_attention_fp4): `k` and
-    `v` are uint8 [H, capacity / 128, bytes of 128 rows], 0.14 of the memory; queries, new rows, outputs and arithmetic stay fp32."""
+    `v` are uint8 [H, capacity / 128, bytes of 128 rows], 0.14 of the memory; queries, new rows, outputs and arithmetic stay fp32.
+
+    The calls on one cache share its workspace: they are ordered, on one stream or by events."""
 
     def __init__(self, heads: int, head_dim: int, device, capacity: int = 1024, kv_bits: int = 32):
         if kv_bits not in (32, 4):
@@ -51,6 +53,10 @@ class DecodeCache:
     @property
     def capacity(self) -> int:
         return self.k.shape[1] * 128 if self.kv_bits == 4 else self.k.shape[0]
+
+    def device_status(self) -> int:
+        """Synchronises and returns the status word of a 4-bit cache's kernels (0 = ok; no other value without a fault of the machine)."""
+        return int(self.workspace[:4].view(torch.int32).item()) if self.kv_bits == 4 else 0
 
     def _grow(self, rows: int) -> None:
         cap = self.capacity
@@ -104,6 +110,8 @@ class DecodeCache:
         n = k.shape[0]
         if tuple(k.shape) != (n, self.heads, self.head_dim) or k.shape != v.shape:
             raise ValueError(f"k and v must be [n, {self.heads}, {self.head_dim}]")
+        if k.dtype != torch.float32 or v.dtype != torch.float32:
+            raise ValueError("k and v must be float32")
         if self.count + n > self.capacity:
             self._grow(self.count + n)
         if self.kv_bits == 4:
@@ -185,7 +193,8 @@ class B200CausalAttention(torch.nn.Module):
 
 def convert_camera_head(head, kv_bits: int = 32) -> int:
     """Switch the attention modules of a CameraCausalHead's trunk (camera_head.py:221-228) to B200CausalAttention, whose caches are held
-    in fp32 or (kv_bits=4) in 4 bits.  Returns how many were converted."""
+    in fp32 or (kv_bits=4) in 4 bits; modules that are converted already take the new kv_bits for the caches they create from now on.
+    Returns how many were converted."""
     if kv_bits not in (32, 4):
         raise ValueError(f"kv_bits must be 32 (fp32) or 4, got {kv_bits!r}")
     n = 0
@@ -193,6 +202,7 @@ def convert_camera_head(head, kv_bits: int = 32) -> int:
         attn = getattr(blk, "attn", None)
         if attn is not None and hasattr(attn, "qkv") and hasattr(attn, "gate_proj") and not isinstance(attn, B200CausalAttention):
             attn.__class__ = B200CausalAttention
-            attn.b200_kv_bits = kv_bits
             n += 1
+        if isinstance(attn, B200CausalAttention):
+            attn.b200_kv_bits = kv_bits
     return n

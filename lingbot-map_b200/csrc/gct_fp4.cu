@@ -778,8 +778,8 @@ int launch_fp4_read(const Fp4ReadLaunch& p, cudaStream_t stream) {
 
 int launch_fp4_rows_append(const float* k, const float* v, int rows, uint8_t* cache_k, uint8_t* cache_v, const Fp4Layout& layout, int first, int heads,
                            int head_dim, cudaStream_t stream) {
-  if (k == nullptr || v == nullptr || cache_k == nullptr || cache_v == nullptr || rows < 0 || first < 0 || heads <= 0 || layout.tail_rows != 0 ||
-      (head_dim != 64 && head_dim != 128))
+  if ((rows > 0 && (k == nullptr || v == nullptr)) || cache_k == nullptr || cache_v == nullptr || rows < 0 || first < 0 || heads <= 0 ||
+      layout.tail_rows != 0 || (head_dim != 64 && head_dim != 128))
     return fail(GCT_ERR_INVALID, "fp4 append: bad argument");
   if (misaligned16(k) || misaligned16(v) || misaligned16(cache_k) || misaligned16(cache_v)) return fail(GCT_ERR_INVALID, "fp4 append: tensors must be 16-byte aligned");
   if (static_cast<int64_t>(first) + rows > static_cast<int64_t>(layout.full_blocks) * kFp4Rows) return fail(GCT_ERR_CAPACITY, "fp4 append: the cache is full");

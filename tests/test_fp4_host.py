@@ -158,3 +158,30 @@ def test_camera_head_conversion_keeps_the_width():
     assert convert_camera_head(head) == 0                   # converted already
     with pytest.raises(ValueError):
         convert_camera_head(head, 8)
+
+
+def test_converted_camera_heads_take_a_new_width():
+    from lingbot_map_b200.camera import convert_camera_head
+
+    class Attn(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.qkv, self.gate_proj = torch.nn.Linear(2, 2), None
+
+    head, blk = torch.nn.Module(), torch.nn.Module()
+    blk.attn = Attn()
+    head.trunk = torch.nn.ModuleList([blk])
+    assert convert_camera_head(head) == 1 and blk.attn.b200_kv_bits == 32
+    assert convert_camera_head(head, 4) == 0 and blk.attn.b200_kv_bits == 4
+
+
+def test_appends_of_no_rows_and_of_other_types():
+    lib = _lib.load()
+    one = 4096
+    assert lib.gct_decode_append_fp4(None, None, 0, one, one, 5, 128, 2, 64, None) == _lib.GCT_OK
+    assert lib.gct_decode_append_fp4(None, one, 1, one, one, 5, 128, 2, 64, None) == _lib.ERR_INVALID
+    for bits in (4, 32):
+        c = P.DecodeCache(2, 64, "cpu", capacity=128, kv_bits=bits)
+        with pytest.raises(ValueError):
+            c.append(torch.zeros(1, 2, 64, dtype=torch.float64), torch.zeros(1, 2, 64))
+        assert c.count == 0 and c.device_status() == 0

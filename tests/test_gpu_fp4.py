@@ -604,3 +604,16 @@ def test_attention_captured_into_a_graph():
             want, _, weighted = F.attention(x, k, v)
             assert (np.abs(host(out) - want) <= bound_frame(len(k), spread_of(x, k), weighted, want)).all()
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [4, 32])
+def test_appends_of_no_rows(bits):
+    c = P.DecodeCache(2, 64, DEV, kv_bits=bits)
+    none = torch.zeros(0, 2, 64, device=DEV)
+    c.append(none, none)
+    one = torch.ones(1, 2, 64, device=DEV)
+    c.append(one, one)
+    c.append(none, none)
+    # two equal rows: their mean is what one of them is held as; in 4 bits 1 / 6 rounds to the scale 0.171875, of which it is 5.8 times, held as 6 times
+    want = 6 * 0.171875 if bits == 4 else 1.0
+    assert c.count == 1 and c.device_status() == 0 and torch.equal(c.attend(one, one, one, False), one * want)
