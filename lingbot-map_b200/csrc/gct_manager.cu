@@ -315,7 +315,10 @@ int gct_mgr_bind(gct_mgr_t* m, void* const* pools_dev, void* workspace_dev, size
   m->part_floats = avail / sizeof(float);
   m->rows_counters = m->fp4 ? reinterpret_cast<int*>(m->ws + w.counters_off) : nullptr;
   GCT_CUDA_CHECK(cudaMemset(m->ws, 0, kWsHeader));
-  if (m->fp4) GCT_CUDA_CHECK(cudaMemset(m->rows_counters, 0, kRowsCounters * sizeof(int)));
+  if (m->fp4) {
+    GCT_CUDA_CHECK(cudaMemset(m->rows_counters, 0, kRowsCounters * sizeof(int)));
+    GCT_CUDA_CHECK(cudaStreamSynchronize(nullptr));      // the counters are zero for the first call on any stream
+  }
   const size_t kn_bytes = static_cast<size_t>(m->cfg.num_blocks) * H * sizeof(float);
   m->key_norm_max = kWsKeyNormOff + kn_bytes <= kWsHeader ? reinterpret_cast<float*>(m->ws + kWsKeyNormOff) : nullptr;
   // nothing is visible yet and the header was just zeroed: a maximum of 0 is exact
