@@ -794,8 +794,10 @@ static int timed_attention(gct_mgr* m, int block, const AttnLaunch& a, bool with
 
 extern "C" {
 
-// Query rows up to which a call over a 4-bit cache takes the kernel for few rows.
-static constexpr int kRowsMaxQueries = 16;
+// Query rows up to which a call over a 4-bit cache takes the kernel for few rows, which goes over K and V once for eight of them; the tile kernel takes
+// the same time for one as for 128.  us at 2 / 9 / 1,017 / 10,000 frames of 1005 tokens, 16 heads: few rows 16 rows 8.9 / 12.8 / 49 / 76, 24 rows
+// 9.5 / 15.0 / 68 / 107, 32 rows 9.1 / 16.8 / 87 / 141; tiles 12.4 / 19.6 / 79 / 126 for any of them.
+static constexpr int kRowsMaxQueries = 24;
 
 // A few query rows over a 4-bit cache; every result is final: splits_out != nullptr leaves it as the one partial result.
 static int run_paged_fp4(gct_mgr* m, int block, const void* q_dev, int q_dtype, int n_q, __nv_bfloat16* out_bf16, float* out_f32, float* lse_dev,

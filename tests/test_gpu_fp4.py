@@ -617,3 +617,21 @@ def test_appends_of_no_rows(bits):
     # two equal rows: their mean is what one of them is held as; in 4 bits 1 / 6 rounds to the scale 0.171875, of which it is 5.8 times, held as 6 times
     want = 6 * 0.171875 if bits == 4 else 1.0
     assert c.count == 1 and c.device_status() == 0 and torch.equal(c.attend(one, one, one, False), one * want)
+
+
+@pytest.mark.parametrize("patches,H,frames,scale,window", [(27, 2, 290, 2, 280), (20, 3, 9, 2, 4), (300, 2, 5, 2, 4)])
+def test_query_tiles_of_few_rows_and_many_pages(patches, H, frames, scale, window):
+    """Around the number of rows from which on a call takes the tile kernel; the first case has more pages than a plan hands over as an argument."""
+    T = patches + NS
+    rs = np.random.RandomState(frames)
+    m, k, v = filled(T, H, frames, rs, scale=scale, window=window)
+    assert (len(m.build_visible_page_table(0)) > 256) == (frames == 290)
+    for n_q in (23, 24, 25, 26, T):
+        q = bf(rs.standard_normal((n_q, H, 64)) * 2)
+        want, want_lse, weighted = F.attention(q, k, v)
+        out, lse = m.compute_attention(0, dev(q, torch.bfloat16), return_lse=True)
+        tol = bound_frame(len(k), spread_of(q, k), weighted, want)
+        assert (np.abs(host(out) - want) <= tol).all()
+        assert np.abs(host(lse) - want_lse).max() <= 2.0 ** -16 * spread_of(q, k) + 2.0 ** -13 + len(k) * 2.0 ** -23
+        assert (np.abs(host(m.compute_attention(0, dev(q, torch.bfloat16))) - want) <= tol).all()
+    assert m.device_status() == 0
