@@ -10,7 +10,8 @@
 //   softmax warps      as there, 32 columns of S at a time, so that 88 registers do (64 at a time spilled: 10 % slower)
 //
 // A value costs its unpacking once per CTA, for the 256 query rows of two tiles: 16,384 values a block, about 800 of the block's 6,100 warp
-// instructions.  1005 queries over 131,928 tokens, kernel and merge back to back: 650 us (840 TFLOP/s; the bf16 cache 559); with four unpacking
+// instructions.  1005 queries over 131,928 tokens, kernel and merge back to back: 628 us in a burst (865 TFLOP/s, 0.51 of a library product's rate;
+// the bf16 cache 559), 662 under the power cap.  As the steps were made, nine equal ranges: 650 us; with four unpacking
 // warps 692, without the fifth K16 step (below) 688, unpacking by the softmax warps between their blocks 742, without any unpacking (wrong
 // results) 647 when the whole took 692.  What bounds it: as in gct_attn_kernel issue slots (packed f32x2 operations take two each) and the
 // chain S -> registers -> P -> P V; issue 64 % busy, tensor pipe 48 %.

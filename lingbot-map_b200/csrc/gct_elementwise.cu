@@ -67,7 +67,8 @@ __device__ __forceinline__ float row_sum(float x) {
 // type at each load makes the loads wait for one another; norm parameters are read once per CTA into shared memory under the
 // row loads.  With eight lanes per row and types at
 // run time (31 shuffles per four heads instead of 10 per eight, three round trips in a row) one frame took 8.5 us (2-D) and 9.9 us (3-D,
-// pages), now 6.0 and 6.4 us; eight frames (99 MB) 31.5 us, now 21.2 us (4.7 TB/s).
+// pages), now 6.0 and 6.4 us; eight frames (99 MB) 31.5 us, now 21.2 us (4.7 TB/s).  Into a 4-bit cache one frame takes 6.7 us where the bf16
+// cache takes 5.6 (one box, back to back): the maximum and the quotients of K and V stand between the loads and the stores.
 constexpr int kPrepThreads = 128;
 constexpr int kRope3dF64 = 3;            // GCT_ROPE_3D on a table of doubles
 

@@ -137,9 +137,14 @@ __global__ void __launch_bounds__(128) gct_fp4_rows_append_kernel(const float* _
 //    t+8, t+12: keys are numbered so that the logits of a lane's query are, without an exchange, the right operand of (p v)^T.
 //  * V's operand pairs two keys at one d.  Two words of two keys are woven into words whose bytes hold (key a, key b) with two logical
 //    operations and a shift each, before a single conversion makes the pair; a weave after the conversion costs twice that.
+//
+// One query over 131,928 tokens of 16 heads (152 MB) 39.7 us, 3.8 TB/s, 0.59 of a copy's rate; eight 44.4; one over 10,000 cached rows of
+// 16 heads with D = 128 (23 MB, from L2) 12.0 us.  Issue slots bound the first (61 % busy; the copies alone take 29.5 us); the second is a start,
+// five blocks or fewer per CTA, and the join of the ranges (9.8 us without computing anything).
 constexpr int kRowsWarps = 4;
 // Keys of a block that a warp takes per turn.  64: two pairs of warps take blocks by turns, which halves what a warp does once per turn (the
-// wait, maximum, vote and shift: some seventy instructions beside five a key); one query over 131,928 tokens 60.5 us with 32, 47.8 with 64.
+// wait, maximum, vote and shift: some seventy instructions beside five a key); when it was chosen, one query over 131,928 tokens 60.5 us with 32,
+// 47.8 with 64.
 // 32: all four warps share a block; right for the camera head's short ranges of a few blocks per CTA (1,000 cached tokens 9.2 us, with 64 11.9).
 template <bool kPaged>
 constexpr int kTurnKeys = kPaged ? 64 : 32;
@@ -147,7 +152,7 @@ constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr float kWeightShift = 15.f;       // weights are at most 2^15
 
 // CTAs that share an SM: five warps of 96 (128) registers each, and 41 (74) KB.  Five CTAs at D = 64 (72 registers, 32 bytes spilled): one query
-// over 131,928 tokens 50.6 us, with four 46.4.
+// over 131,928 tokens 50.6 us, with four 46.4 (before the last steps on either).
 template <int D>
 constexpr int kRowsCtas = D == 64 ? 4 : 3;
 
