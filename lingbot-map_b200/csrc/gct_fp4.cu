@@ -206,6 +206,9 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
   rest = pack_f16x2(x - f.x, y - f.y);
 }
 
+// Ranges in flight where they are joined: with five, eight queries at D = 128 took 4 us longer, with 13 up to 1.5 us.
+constexpr int kJoinAhead = 9;
+
 template <int D, bool kPaged>
 __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kernel(const RowsArgs a, const __grid_constant__ Fp4Pages pages) {
   using L = RowsSmem<D, kPaged>;
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<D>) gct_fp4_rows_kerne
   // maximum among them, then they are joined in order.  Maxima and sums come in one trip.
   float4* lane_sum = reinterpret_cast<float4*>(smem);
   const float* recs = a.part + item * a.splits * 8 * kRecord;
-  constexpr int kCols = D / 4, kAhead = 9;                 // ranges in flight: with five, eight queries at D = 128 took 4 us longer
+  constexpr int kCols = D / 4, kAhead = kJoinAhead;
   const int items = rows_here * kCols;
   int lanes = 1;
   while (2 * lanes * items <= 128) lanes *= 2;
@@ -690,13 +693,33 @@ bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 
 }  // namespace
 
-int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters) {
-  const int64_t items = static_cast<int64_t>(groups) * heads;
+// More ranges share the keys among more CTAs of an SM, and make the join longer, which one CTA per (head, eight queries) does in trips to L2.  As
+// many as fill one, two, ... CTAs per SM are compared, in hundredths of a us as measured: a trip, and a block at so many CTAs per SM.  us with
+// 9 / 18 / 37 ranges (one, two, four CTAs), 16 heads of 64: eight queries over 33 blocks 8.6 / 9.1 / 10.2, 81 blocks 10.6 / 10.3 / 11.6, 161 blocks
+// 14.9 / 13.4 / 15.1; six over 181 blocks 16.4 / 14.3 / 14.7, 625 blocks 40.8 / 31.1 / 29.8; one over 81 blocks 10.0 / 9.0 / 8.1.  With 9 / 18 / 27 ranges of
+// 16 heads of 128: eight over 24 blocks 11.9 / 15.1 / 14.9, 79 blocks 17.8 / 20.7 / 18.7; one over 79 blocks 14.9 / 14.9 / 12.0.
+int fp4_rows_splits(int n_q, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters) {
+  constexpr int kTrip = 80, kBlock64[kRowsCtas<64>] = {50, 68, 110, 105}, kBlock128[kRowsCtas<128>] = {98, 180, 200};
+  const int64_t items = static_cast<int64_t>((n_q + 7) / 8) * heads;
   if (blocks <= 1 || items > num_counters) return 1;
-  const int64_t slots = static_cast<int64_t>(sms) * (head_dim == 64 ? kRowsCtas<64> : kRowsCtas<128>);
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / items, blocks));
-  splits = std::min<int64_t>(splits, static_cast<int64_t>(part_floats / (static_cast<size_t>(items) * 8 * (head_dim == 64 ? kRowsRecord<64> : kRowsRecord<128>))));
-  return static_cast<int>(std::max<int64_t>(splits, 1));
+  const int most_ctas = head_dim == 64 ? kRowsCtas<64> : kRowsCtas<128>, record = head_dim == 64 ? kRowsRecord<64> : kRowsRecord<128>;
+  const int64_t most = std::min<int64_t>(blocks, static_cast<int64_t>(part_floats / (static_cast<size_t>(items) * 8 * record)));
+  const int columns = std::min(n_q, 8) * (head_dim / 4);
+  int lanes = 1;                                           // that share the ranges of four columns of a row, as in the kernel
+  while (2 * lanes * columns <= 128) lanes *= 2;
+  const int passes = (columns * lanes + kRowsThreads - 1) / kRowsThreads;
+  int64_t best = 1, best_cost = -1;
+  for (int ctas = most_ctas; ctas >= 1; --ctas) {
+    const int64_t splits = std::max<int64_t>(1, std::min(most, static_cast<int64_t>(sms) * ctas / items));
+    const int64_t per_sm = std::min<int64_t>(most_ctas, (splits * items + sms - 1) / sms);
+    const int64_t trips = passes * ((splits + kJoinAhead * lanes - 1) / (kJoinAhead * lanes));
+    const int64_t cost = kTrip * trips + (blocks + splits - 1) / splits * (head_dim == 64 ? kBlock64 : kBlock128)[per_sm - 1];
+    if (best_cost < 0 || cost < best_cost) {
+      best = splits;
+      best_cost = cost;
+    }
+  }
+  return static_cast<int>(best);
 }
 
 int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream) {
@@ -745,7 +768,7 @@ int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream) {
   int sms = 148;
   const int rc = device_sm_count(&sms);
   if (rc != GCT_OK) return rc;
-  k.splits = p.counters == nullptr || p.part == nullptr ? 1 : fp4_rows_splits(k.groups, p.heads, k.blocks, p.head_dim, sms, p.part_floats, p.num_counters);
+  k.splits = p.counters == nullptr || p.part == nullptr ? 1 : fp4_rows_splits(p.n_q, p.heads, k.blocks, p.head_dim, sms, p.part_floats, p.num_counters);
   k.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
   k.out_bf16 = p.out_bf16;
   k.out_f32 = p.out_f32;

@@ -171,7 +171,7 @@ int launch_fp4_rows(const Fp4RowsLaunch& p, cudaStream_t stream);
 // page_ids: as for Fp4RowsLaunch; exact_logits: for callers who want the log-sum-exp.
 int launch_attention_fp4(const AttnLaunch& a, const uint8_t* pool, const Fp4Layout& layout, int num_pages, const int32_t* page_ids, bool exact_logits,
                          cudaStream_t stream);
-// Key ranges that a call of `groups` x `heads` (head, eight queries) items over `blocks` blocks of 128 rows is cut into.
-int fp4_rows_splits(int groups, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters);
+// Key ranges that a call of n_q query rows of `heads` heads over `blocks` blocks of 128 rows is cut into.
+int fp4_rows_splits(int n_q, int heads, int blocks, int head_dim, int sms, size_t part_floats, int num_counters);
 
 }  // namespace gct
