@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(128) gct_fp4_rows_append_kernel(const float* _
 //    [2^14, 2^15) by a power of two per row) at the price of one.  (p v)^T has d as its rows and the queries as its eight columns, once with
 //    the weights exp2(x - max + 15) and once with their rests.  Results agree with fp32 arithmetic to about 2^-21.  With the queries as rows
 //    of p v its sums took twice the registers.  The paged cache's calls take bf16 queries, which leave no rest, and give bf16 results, for
-//    which a weight's eleven bits are enough (2^-12 of sum p |v|, a sixteenth of the result's own rounding): no rests there.
+//    which a weight's eleven bits are enough (at most 2^-11 of sum p |v|, an eighth of the result's own rounding): no rests there.
 //  * Any order of d is right for q k^T and any order of keys and of d for p v, as long as both operands agree.  A lane takes a
 //    quarter row of K as one 8- or 16-byte load (the d that it multiplies are its own), and of V an eighth of a row of the keys t, t+4,
 //    t+8, t+12: keys are numbered so that the logits of a lane's query are, without an exchange, the right operand of (p v)^T.

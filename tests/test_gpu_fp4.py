@@ -45,13 +45,14 @@ def same_rows(got, x, tag):
 
 
 def bound_rows(keys, spread, weighted, out):
-    """Few-row kernel, a bf16 result `out` of float64: the final rounding is half a step, 2^-8 |out|.  A logit's error: q enters with 22 bits,
-    products are exact, fp32 sums of at most 128 terms: below (2^-22 + 128 * 2^-24) * sum |q k| / sqrt(D) <= 2^-16 * `spread`; times ln 2 either way
-    it moves a weight by that much relatively; exp2 and the two-part weight add 2^-21; fp32 sums over the keys keys * 2^-24 (each addition rounds
+    """Few-row kernel, a bf16 result `out` of float64: the final rounding is half a step, 2^-8 |out|.  A logit's error: q, bf16, is exact in half
+    precision, products are exact, fp32 sums of at most 128 terms: below (2^-22 + 128 * 2^-24) * sum |q k| / sqrt(D) <= 2^-16 * `spread`; times ln 2 either way
+    it moves a weight by that much relatively; exp2 adds 2^-21; fp32 sums over the keys keys * 2^-24 (each addition rounds
     or cuts, relative 2^-23 on partial sums).  Relative weight errors move the result by that share of sum p |v| (`weighted`), twice as numerator and
     denominator both carry them.  A weight is held to 2^-40 of the largest (half of half precision's smallest step, 2^-25, at weights of up to
-    2^15): far smaller ones are zero, which moves the result by at most keys * 2^-40 * max|v|, and |v| is below 2^3 in these tests."""
-    return 2.0 ** -8 * np.abs(out) + 2 * (2.0 ** -16 * spread + 2.0 ** -21 + keys * 2.0 ** -23) * weighted + keys * 2.0 ** -37
+    2^15): far smaller ones are zero, which moves the result by at most keys * 2^-40 * max|v|, and |v| is below 2^3 in these tests.  In front of V, not
+    in the sum that divides, a weight is one half-precision number: half a step is 2^-11 of it, which moves the result by at most 2^-11 `weighted`."""
+    return 2.0 ** -8 * np.abs(out) + (2.0 ** -11 + 2 * (2.0 ** -16 * spread + 2.0 ** -21 + keys * 2.0 ** -23)) * weighted + keys * 2.0 ** -37
 
 
 def spread_of(q, k):
@@ -378,7 +379,8 @@ def test_softmax_reference(patches, n_q, regime):
 
 # ---------------------------------------------------------------- the camera head's caches
 def decode_bound(keys, spread, weighted):
-    """fp32 results: as bound_rows without the last rounding; the rounding of the division and of the result, 2^-23, is inside the first terms."""
+    """fp32 results: as bound_rows without the last rounding, and with q and the weights in two parts (22 bits each: 2^-22 of a logit's terms, 2^-22 of a
+    weight); the rounding of the division and of the result, 2^-23, is inside the first terms."""
     return 2 * (2.0 ** -16 * spread + 2.0 ** -20 + keys * 2.0 ** -23) * weighted + 2.0 ** -30
 
 
@@ -634,4 +636,28 @@ def test_query_tiles_of_few_rows_and_many_pages(patches, H, frames, scale, windo
         assert (np.abs(host(out) - want) <= tol).all()
         assert np.abs(host(lse) - want_lse).max() <= 2.0 ** -16 * spread_of(q, k) + 2.0 ** -13 + len(k) * 2.0 ** -23
         assert (np.abs(host(m.compute_attention(0, dev(q, torch.bfloat16))) - want) <= tol).all()
+    assert m.device_status() == 0
+
+
+def test_exchange_with_one_rank():
+    """gct_mgr_attention_exchange with world = 1 takes the partial results of either kernel: one final range of a few rows, several of query tiles."""
+    import ctypes as C
+    from lingbot_map_b200.cache import _stream_ptr
+    lib = _lib.load()
+    rs = np.random.RandomState(21)
+    m, k, v = filled(306, 2, 9, rs)
+    m.plan()
+    one = lambda t: (C.c_void_p * 1)(t.data_ptr())
+    flags = torch.zeros(64, dtype=torch.int32, device=DEV)
+    for epoch, n_q in enumerate((306, 5, 24, 129), 1):
+        rb, fb, sl = C.c_size_t(), C.c_size_t(), C.c_int()
+        _lib.check(lib.gct_kv_exchange_sizes(n_q, 2, 1, C.byref(rb), C.byref(fb), C.byref(sl)))
+        recv = torch.zeros(rb.value // 4, dtype=torch.float32, device=DEV)
+        out = torch.zeros(n_q, 2, 64, dtype=torch.bfloat16, device=DEV)
+        q = bf(rs.standard_normal((n_q, 2, 64)))
+        qd = dev(q, torch.bfloat16)
+        _lib.check(lib.gct_mgr_attention_exchange(m._handle, 0, qd.data_ptr(), _lib.BF16, n_q, 0, 1, 1, one(recv), one(out), one(flags), sl.value, epoch,
+                                                  _stream_ptr(m.device)))
+        want, _, weighted = F.attention(q, k, v)
+        assert (np.abs(host(out) - want) <= bound_frame(len(k), spread_of(q, k), weighted, want)).all()
     assert m.device_status() == 0
