@@ -315,7 +315,8 @@ def test_plans_of_many_pages():
 
 def bound_frame(keys, spread, weighted, out):
     """Any path: as bound_rows, with weights rounded to half precision (2^-11 relative; below 2^-14 of their scale 2^-25 absolutely) and
-    exponentials good to 2^-13 in numerator and denominator, and the merge of ranges in fp32."""
+    exponentials good to 2^-13 in numerator and denominator, and the merge of ranges in fp32.  Where q is rounded once more with its scale (2^-11 of each
+    term of a logit, to either side) nothing is granted for it: the terms cancel."""
     return 2.0 ** -8 * np.abs(out) + (2.0 ** -11 + 2.0 ** -12 + 2 * (2.0 ** -16 * spread + keys * 2.0 ** -23)) * weighted + 2.0 ** -24
 
 
