@@ -10,8 +10,8 @@
 //   softmax warps      as there, 32 columns of S at a time, so that 88 registers do (64 at a time spilled: 10 % slower)
 //
 // A value costs its unpacking once per CTA, for the 256 query rows of two tiles: 16,384 values a block, about 800 of the block's 6,100 warp
-// instructions.  1005 queries over 131,928 tokens, kernel and merge back to back: 628 us in a burst (865 TFLOP/s, 0.51 of a library product's rate;
-// the bf16 cache 559), 662 under the power cap.  As the steps were made, nine equal ranges: 650 us; with four unpacking
+// instructions.  1005 queries over 131,928 tokens, kernel and merge back to back: 621 us in a burst (874 TFLOP/s, 0.51 of a library product's rate;
+// the bf16 cache 559), 656 under the power cap; with the running maximum 932.  As the steps were made, nine equal ranges: 650 us; with four unpacking
 // warps 692, without the fifth K16 step (below) 688, unpacking by the softmax warps between their blocks 742, without any unpacking (wrong
 // results) 647 when the whole took 692.  What bounds it: as in gct_attn_kernel issue slots (packed f32x2 operations take two each) and the
 // chain S -> registers -> P -> P V; issue 64 % busy, tensor pipe 48 %.
@@ -31,7 +31,9 @@ constexpr int kPackedStages = 4, kTileStages = 2;          // blocks (K and V) i
 constexpr uint32_t kPackedBytes = kFp4BlockBytes<64>;
 constexpr float kFp4Shift = 7.f;                           // running maximum: weights are at most 2^(kRescaleThreshold + kFp4Shift)
 constexpr float kFixedShift = 15.f;                        // fixed reference: weights are at most 2^15
-constexpr int kFixedNum = 1, kFixedDen = 4;                // there, pairs of logits whose exponentials take the FMA pipe
+// One pair of logits in so many takes the FMA pipe for its exponentials.  1005 queries over 131,928 tokens, fixed reference / running maximum: three 626 / 951
+// us, four 621 / 935, five 647 / 948, six 654 / 960.
+constexpr int kPolyDen = 4;
 // half-precision operands: formats 0; K-major A and B for S, MN-major B for P V
 constexpr uint32_t kIdescS16 = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescPV16 = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
@@ -39,8 +41,9 @@ constexpr uint32_t kIdescPV16 = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((
 // Warpgroups: two softmax per query tile, one of producer and MMA warps, two that unpack.
 template <int QT>
 constexpr int kFp4Threads = 256 * QT + 384;
-// Two tiles: 896 threads start with 72 registers each, 64512 in all.
-constexpr int kFp4SoftmaxRegs = 88, kFp4ControlRegs = 40, kFp4UnpackRegs = 56;
+// Two tiles: 896 threads start with 72 registers each, 64512 in all.  With 88 / 40 / 56 the control warpgroup spilled (28 bytes): 131,928 tokens 629 us, now 621;
+// 96 / 40 / 40 627, 88 / 56 / 48 641.
+constexpr int kFp4SoftmaxRegs = 88, kFp4ControlRegs = 48, kFp4UnpackRegs = 48;
 static_assert(512 * kFp4SoftmaxRegs + 128 * kFp4ControlRegs + 256 * kFp4UnpackRegs <= 896 * 72, "register pool of the CTA exceeded");
 
 template <int QT>
@@ -448,12 +451,11 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
     const float c = *factor;
     float m = -INFINITY, l = 0.f;                          // m: reference maximum (units of S); l: sum over this half
 
-    // P = exp2(S c + shift) of some logits as half-precision pairs, and their sum, software-pipelined over pairs as in gct_attn_kernel.  kNum of
-    // kDen pairs take the FMA pipe; kBelow: exponents may lie below -126.
-    auto sweep = [&](auto& s, auto& pk, float shift, auto below, auto num, auto den) -> float {
+    // P = exp2(S c + shift) of some logits as half-precision pairs, and their sum, software-pipelined over pairs as in gct_attn_kernel.
+    // kBelow: exponents may lie below -126.
+    auto sweep = [&](auto& s, auto& pk, float shift, auto below) -> float {
       constexpr int kPairs = sizeof(pk) / sizeof(pk[0]);
       constexpr bool kBelow = decltype(below)::value;
-      constexpr int kNum = decltype(num)::value, kDen = decltype(den)::value;
       const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
       float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
       auto pair_ffma = [&](int q) {
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
         s[2 * q + 1] = __float_as_uint(x.y);
       };
       auto pair_exp = [&](int q) {
-        if (((q + 1) * kNum) / kDen != (q * kNum) / kDen) {
+        if ((q + 1) / kPolyDen != q / kPolyDen) {
           const float2 x = make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
           const float2 e = kBelow ? exp2_poly2(x) : exp2_poly2_inrange(x);
           s[2 * q] = __float_as_uint(e.x);
@@ -490,7 +492,6 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
       for (int q = kPairs - kSumLag; q < kPairs; ++q) pair_sum(q);
       return (acc0.x + acc0.y) + (acc1.x + acc1.y);
     };
-    using std::integral_constant;
     using Yes = std::true_type;
     using No = std::false_type;
     auto load_s = [&](int ch, int valid, uint32_t hidden, uint32_t (&s)[32]) {       // 32 columns of this thread's half; `valid` of the 64 count
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
             for (int i = 0; i < 32; ++i)
               if (32 * ch + i >= valid) s[i] = hidden;
           }
-          l += sweep(s, pk, shift, No(), integral_constant<int, kFixedNum>(), integral_constant<int, kFixedDen>());
+          l += sweep(s, pk, shift, No());
           if (ch == 0 && j > 0) {                          // P is free once the product of the block before has read it
             if (!(ok = wait_u(bar_pv_full(t, half), (j - 1) & 1))) break;
             tc_fence_after();
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(kFp4Threads<QT>, 1) gct_attn_fp4_kernel(const 
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - m);
           }
-          l += sweep(s, pk, kFp4Shift - (huge ? 0.f : base), Yes(), integral_constant<int, QT == 2 ? 2 : 1>(), integral_constant<int, QT == 2 ? 7 : 3>());
+          l += sweep(s, pk, kFp4Shift - (huge ? 0.f : base), Yes());
           if (ch == 0 && j > first) {
             if (!(ok = wait_u(bar_pv_full(t, 1), (j - 1) & 1))) break;
             tc_fence_after();
